@@ -234,6 +234,27 @@ int gb_rope_kv_paged_launch(const float *qkv, int T, int q_rows, int kv_rows, in
 int gb_f32_to_f16_launch(const float *x, __half *y, size_t n, cudaStream_t st);
 int gb_argmax_rows_launch(const float *x, int rows, int n, int32_t *out, cudaStream_t st);
 
+// gb_rows.cu: per-head norms, rotation and the append to the pages. Arguments are
+// checked before `loaded` (a handle was given), so refusals need no device.
+int gb_paged_chunk_check(const char *what, const gb_paged_chunk *c);
+int gb_qk_norm_rope_launch(int typ, const void *q, long long ldq, int n_heads, const void *k, long long ldk, int n_kv,
+                           int rows, int head_dim, const gb_qk_norm_params *norm, const gb_rope_params *rope,
+                           const int32_t *pos, int out_typ, void *q_out, long long ldqo, void *k_out, long long ldko,
+                           bool loaded, cudaStream_t st);
+int gb_rope_append_paged_launch(const gb_paged_chunk *c, int typ, const void *q, long long ldq, int n_heads,
+                                const void *k, long long ldk, const void *v, long long ldv,
+                                const gb_qk_norm_params *norm, const gb_rope_params *rope, void *q_out, long long ldqo,
+                                bool loaded, cudaStream_t st);
+
+// gb_chunk.cu: attention of a batch's new rows over the pages. The check is
+// apart from the launch: it needs no device.
+size_t gb_attn_chunk_part_floats(int sms);
+int gb_attn_chunk_counters(int sms);
+int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale,
+                        const void *out, long long ldo);
+int gb_attn_chunk_launch(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale, void *out,
+                         long long ldo, float *part, unsigned *counter, int sms, cudaStream_t st);
+
 // gb_sample.cu: one token from logits[n]; parameters by value (p_host) or
 // from device memory (p_dev, for graph replays); the penalty window is
 // recent[n_recent] or, for the model, fed[pos-N+1..pos]; counter = *pos when

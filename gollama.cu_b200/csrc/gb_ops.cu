@@ -497,6 +497,8 @@ struct gb_kernels {
   size_t pws_floats = 0;
   unsigned *pws_counter = nullptr;
   size_t pws_counters = 0;
+  float *cws = nullptr;  // chunk attention: partial rows + counters, one allocation of a fixed size
+  int sms = 0;
 };
 
 // The kernel names backend/gpu binds (backend/gpu/gpu.go:24); each has an
@@ -526,6 +528,7 @@ int gb_gpu_load(int device, gb_kernels **out) {
   GB_CUDA(cudaFuncGetAttributes(&fa, rmsnorm_kernel), "gpu: load kernels");
   gb_kernels *k = new gb_kernels();
   k->device = device;
+  k->sms = prop.multiProcessorCount;
   cudaError_t e = cudaMalloc(&k->status, sizeof(unsigned));
   if (e == cudaSuccess) e = cudaMemset(k->status, 0, sizeof(unsigned));
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -547,10 +550,25 @@ int gb_gpu_close(gb_kernels *k) {
   if (k->ws_counter) cudaFree(k->ws_counter);
   if (k->pws) cudaFree(k->pws);
   if (k->pws_counter) cudaFree(k->pws_counter);
+  if (k->cws) cudaFree(k->cws);
   if (k->status) cudaFree(k->status);
   delete k;
   return GB_OK;
 }
+
+// The handle's device for the length of a call, the caller's afterwards.
+struct OnDevice {
+  int was = -1;
+  explicit OnDevice(const gb_kernels *k) {
+    int cur = 0;
+    if (!k) return;
+    const int device = k->device;
+    if (cudaGetDevice(&cur) == cudaSuccess && cur != device && cudaSetDevice(device) == cudaSuccess) was = cur;
+  }
+  ~OnDevice() {
+    if (was >= 0) cudaSetDevice(was);
+  }
+};
 
 #define GB_NEED(k)                                                        \
   do {                                                                    \
@@ -951,6 +969,55 @@ int gb_gpu_attn_decode_paged(gb_kernels *k, void *stream, const float *q, const 
   return gb_attn_paged_launch(q, k_pool, v_pool, kv_f16, block_table, seq_lens, batch, max_pages, n_pages, page_size,
                               n_heads, n_kv, head_dim, scale, out, nullptr, k->pws, k->pws_counter, (int)S, nullptr,
                               (cudaStream_t)stream);
+}
+
+int gb_gpu_qk_norm_rope(gb_kernels *k, void *stream, int typ, const void *q, int64_t ldq, int n_heads, const void *kx,
+                        int64_t ldk, int n_kv, int rows, int head_dim, const gb_qk_norm_params *norm,
+                        const gb_rope_params *rope, const int32_t *pos, int out_typ, void *q_out, int64_t ldqo,
+                        void *k_out, int64_t ldko) {
+  gb_clear_error();
+  const OnDevice on(k);
+  return gb_qk_norm_rope_launch(typ, q, ldq, n_heads, kx, ldk, n_kv, rows, head_dim, norm, rope, pos, out_typ, q_out,
+                                ldqo, k_out, ldko, k != nullptr, (cudaStream_t)stream);
+}
+
+int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, int typ, const void *q, int64_t ldq,
+                             int n_heads, const void *kx, int64_t ldk, const void *v, int64_t ldv,
+                             const gb_qk_norm_params *norm, const gb_rope_params *rope, void *q_out, int64_t ldqo) {
+  gb_clear_error();
+  const OnDevice on(k);
+  return gb_rope_append_paged_launch(c, typ, q, ldq, n_heads, kx, ldk, v, ldv, norm, rope, q_out, ldqo,
+                                     k != nullptr, (cudaStream_t)stream);
+}
+
+int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, const void *q, int64_t ldq,
+                            int n_heads, float scale, void *out, int64_t ldo) {
+  gb_clear_error();
+  const int rc = gb_attn_chunk_check(c, q, ldq, n_heads, scale, out, ldo);
+  if (rc != GB_OK) return rc;
+  GB_NEED(k);
+  if (!c->rows || !c->batch) return GB_OK;
+  const OnDevice on(k);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const size_t floats = gb_attn_chunk_part_floats(k->sms);
+  if (!k->cws) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    GB_CUDA(cudaStreamIsCapturing(st, &cap), "gpu: chunk attention");
+    if (cap != cudaStreamCaptureStatusNone)
+      return gb_fail(GB_ERR_INVALID, "gpu: chunk attention: the handle's first call allocates: make it before a capture");
+    const size_t counters = (size_t)gb_attn_chunk_counters(k->sms) * sizeof(unsigned);
+    float *ws = nullptr;
+    GB_CUDA(cudaMalloc(&ws, floats * sizeof(float) + counters), "gpu: chunk attention: workspace");
+    // counters zero before this call's launch, and before any other stream's
+    cudaError_t e = cudaMemsetAsync(ws + floats, 0, counters, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) {
+      cudaFree(ws);
+      return gb_cuda_fail(e, "gpu: chunk attention: workspace");
+    }
+    k->cws = ws;
+  }
+  return gb_attn_chunk_launch(c, q, ldq, n_heads, scale, out, ldo, k->cws, (unsigned *)(k->cws + floats), k->sms, st);
 }
 
 // model.Argmax, model/model.go:376.

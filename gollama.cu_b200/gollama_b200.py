@@ -72,8 +72,47 @@ def sample_params(temperature=0.8, top_k=40, top_p=0.95, repeat_penalty=1.0, rep
     return SampleParams(temperature, top_k, top_p, repeat_penalty, repeat_last_n, 0, seed)
 
 
+class RopeParams(C.Structure):
+    """gb_rope_params: the rotation of a head's first dims elements."""
+    _fields_ = [("base", C.c_float), ("dims", C.c_int), ("halves", C.c_int), ("freq", C.c_void_p)]
+
+
+class QkNormParams(C.Structure):
+    """gb_qk_norm_params: the weights of the per-head query and key norms."""
+    _fields_ = [("wq", C.c_void_p), ("wk", C.c_void_p), ("eps", C.c_float)]
+
+
+class PagedChunk(C.Structure):
+    """gb_paged_chunk: a batch's new rows and the paged cache they belong to."""
+    _fields_ = [(n, C.c_int) for n in ("rows", "batch", "max_pages", "n_pages", "page_size", "n_kv", "head_dim",
+                                        "kv_typ")] + \
+               [(n, C.c_void_p) for n in ("q_start", "kv_lens", "block_table", "k_pool", "v_pool")]
+
+
+def rope(base: float, dims: int, halves: bool = False, freq=None) -> RopeParams:
+    r = RopeParams(base, dims, int(halves), _ptr(freq))
+    r._keep = (freq,)  # the buffers it names live as long as it does
+    return r
+
+
+def qk_norm(wq, wk, eps: float) -> QkNormParams:
+    r = QkNormParams(_ptr(wq), _ptr(wk), eps)
+    r._keep = (wq, wk)
+    return r
+
+
+def paged_chunk(rows, batch, q_start, kv_lens, block_table, max_pages, n_pages, page_size, n_kv, head_dim, kv_typ,
+                k_pool, v_pool) -> PagedChunk:
+    """The description gb_gpu_rope_append_paged and gb_gpu_attn_chunk_paged share; a program keeps one while its
+    buffers stay in place and rewrites their contents from step to step."""
+    r = PagedChunk(rows, batch, max_pages, n_pages, page_size, n_kv, head_dim, kv_typ, _ptr(q_start), _ptr(kv_lens),
+                   _ptr(block_table), _ptr(k_pool), _ptr(v_pool))
+    r._keep = (q_start, kv_lens, block_table, k_pool, v_pool)
+    return r
+
+
 _lib = None
-P, I, U64, F, D, S = C.c_void_p, C.c_int, C.c_uint64, C.c_float, C.c_double, C.c_size_t
+P, I, I64, U64, F, D, S = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_double, C.c_size_t
 _SIGS = {
     "gb_last_error": (C.c_char_p, []), "gb_version": (C.c_char_p, []),
     "gb_gpu_load": (I, [I, C.POINTER(P)]), "gb_gpu_len": (I, [P]), "gb_gpu_close": (I, [P]),
@@ -89,6 +128,9 @@ _SIGS = {
     "gb_gpu_peer_resid": (I, [P, P, I, P, P, P, I, I, P, I, P, C.c_uint, P]),
     "gb_gpu_peer_resid_tagged": (I, [P, P, I, P, P, I, I, P, I, P, C.c_uint, P]), "gb_gpu_sample": (I, [P, P, P, I, P, P, I, U64, P]),
     "gb_gpu_attn_decode_paged": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, F, P]),
+    "gb_gpu_qk_norm_rope": (I, [P, P, I, P, I64, I, P, I64, I, I, I, P, P, P, I, P, I64, P, I64]),
+    "gb_gpu_rope_append_paged": (I, [P, P, P, I, P, I64, I, P, I64, P, I64, P, P, P, I64]),
+    "gb_gpu_attn_chunk_paged": (I, [P, P, P, P, I64, I, F, P, I64]),
     "gb_model_set_sampler": (I, [P, P]), "gb_model_prefill": (I, [P, P, I, I, P]),
     "gb_model_cache_f16_weights": (I, [P, C.POINTER(S)]),
     "gb_linear_matmul_f16": (I, [P, P, P, I, P]), "gb_linear_cache_f16_weights": (I, [P, C.POINTER(S)]),
@@ -167,6 +209,10 @@ def _ptr(x) -> int | None:
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot pass {type(x)} as a pointer")
+
+
+def _ref(x):
+    return None if x is None else C.byref(x)
 
 
 def _stream(s) -> int | None:
@@ -258,6 +304,25 @@ class Kernels:
         _check(lib().gb_gpu_attn_decode_paged(self.h, _stream(stream), _ptr(q), _ptr(k_pool), _ptr(v_pool),
                                               int(kv_f16), _ptr(block_table), _ptr(seq_lens), batch, max_pages,
                                               n_pages, page_size, n_heads, n_kv, head_dim, scale, _ptr(out)))
+
+    def qk_norm_rope(self, typ, q, ldq, n_heads, k, ldk, n_kv, rows, head_dim, norm: QkNormParams | None,
+                     rope: RopeParams | None, pos, out_typ, q_out, ldqo, k_out, ldko, stream=None):
+        """gb_gpu_qk_norm_rope: per-head norms of queries and keys with the rotation in the same pass."""
+        _check(lib().gb_gpu_qk_norm_rope(self.h, _stream(stream), typ, _ptr(q), ldq, n_heads, _ptr(k), ldk, n_kv,
+                                         rows, head_dim, _ref(norm), _ref(rope), _ptr(pos), out_typ, _ptr(q_out), ldqo,
+                                         _ptr(k_out), ldko))
+
+    def rope_append_paged(self, chunk: PagedChunk, typ, q, ldq, n_heads, k, ldk, v, ldv, rope: RopeParams | None,
+                          q_out, ldqo, norm: QkNormParams | None = None, stream=None):
+        """gb_gpu_rope_append_paged: the new rows' keys and values into their pages, rotated on the way, and the
+        rotated queries into q_out."""
+        _check(lib().gb_gpu_rope_append_paged(self.h, _stream(stream), _ref(chunk), typ, _ptr(q), ldq, n_heads,
+                                              _ptr(k), ldk, _ptr(v), ldv, _ref(norm), _ref(rope), _ptr(q_out), ldqo))
+
+    def attn_chunk_paged(self, chunk: PagedChunk, q, ldq, n_heads, scale, out, ldo, stream=None):
+        """gb_gpu_attn_chunk_paged: attention of the new rows over their sequences' pages."""
+        _check(lib().gb_gpu_attn_chunk_paged(self.h, _stream(stream), _ref(chunk), _ptr(q), ldq, n_heads, scale,
+                                             _ptr(out), ldo))
 
     def sample(self, logits, n, params: SampleParams, recent, n_recent, counter, out, stream=None):
         _check(lib().gb_gpu_sample(self.h, _stream(stream), _ptr(logits), n, C.byref(params),

@@ -167,6 +167,83 @@ int gb_gpu_peer_resid_tagged(gb_kernels *k, void *stream, int world, const unsig
                              const unsigned *step, int slot, int dim, float *x, int n, float *ssq,
                              unsigned wait_limit, unsigned *status);
 
+/* ---- new rows over a paged cache (added; the reference's roadmap "Paged KV
+ * cache plus continuous batching", ROADMAP.md:197-202) ----------------------
+ * The calls of one serving step on a batch whose sequences each bring some new
+ * rows (one when decoding, a prompt chunk otherwise): per-head norms and the
+ * rotation, the append of keys and values to the pages, and the attention of
+ * the new rows. Types are GB_F32, GB_F16 or GB_BF16. Every operand lies on a
+ * 16-byte boundary with its rows (tokens) ld* elements apart, a multiple of 8;
+ * a row's heads are contiguous. Launches go to `stream` on the device of `k`,
+ * whichever device is current. */
+
+/* The rotation (cpu.RoPE, backend/cpu/cpu.go:118): the first `dims` elements
+ * of a head (a multiple of 16; 0: none) in pairs (2j, 2j+1), or (j, j + dims/2)
+ * with `halves`, turned by pos * base^(-2j/dims) / freq[j]; freq[dims/2] on the
+ * device, NULL for ones. Angles are formed in float64. */
+typedef struct {
+  float base;
+  int dims;
+  int halves;
+  const float *freq;
+} gb_rope_params;
+
+/* Norms of queries and keys for each head: x * w / sqrt(mean(x^2) + eps), with
+ * w[head_dim] float32 on the device shared by the heads; a NULL weight leaves
+ * the queries (or keys) as they are. */
+typedef struct {
+  const float *wq, *wk;
+  float eps;
+} gb_qk_norm_params;
+
+/* A batch's new rows and the paged cache they belong to. Sequence b's new rows
+ * are rows [q_start[b], q_start[b+1]) of the call's `rows` (q_start[batch+1] on
+ * the device, not decreasing; rows outside [q_start[0], q_start[batch]) belong
+ * to no sequence and their outputs are left as they were). kv_lens[b] counts
+ * its positions WITH the new rows: the i-th of n rows stands at position
+ * kv_lens[b] - n + i. Pools and table are those of gb_gpu_attn_decode_paged:
+ * k_pool / v_pool = [n_pages][n_kv][page_size][head_dim] of type kv_typ,
+ * block_table[batch][max_pages]. */
+typedef struct {
+  int rows, batch, max_pages, n_pages, page_size, n_kv, head_dim, kv_typ;
+  const int32_t *q_start, *kv_lens, *block_table;
+  void *k_pool, *v_pool;
+} gb_paged_chunk;
+
+/* Norms of queries and keys for each head with the rotation in the same pass:
+ * `rows` rows of n_heads query heads (q, type typ) and n_kv key heads (k) to
+ * q_out and k_out (type out_typ), row r at position pos[r] (device; may be
+ * NULL without rotation). norm or rope may be NULL (none); either head count
+ * may be 0. head_dim is a multiple of 16 up to 256. An output may be its own
+ * input (same type and row distance); other overlaps are not allowed. */
+int gb_gpu_qk_norm_rope(gb_kernels *k, void *stream, int typ, const void *q, int64_t ldq, int n_heads, const void *kx,
+                        int64_t ldk, int n_kv, int rows, int head_dim, const gb_qk_norm_params *norm,
+                        const gb_rope_params *rope, const int32_t *pos, int out_typ, void *q_out, int64_t ldqo,
+                        void *k_out, int64_t ldko);
+/* Append the new rows' keys and values (type typ, rounded to the pool's) to
+ * the cache at their positions, the keys normed and rotated on the way (norm,
+ * rope: NULL for none), and the queries with them into q_out (the pool's type;
+ * n_heads 0: no queries). A row whose position is negative or past the table,
+ * or whose page is outside [0, n_pages), is not appended (its query is still
+ * written). Slots no row is appended to keep their contents. Two rows must not
+ * share a slot. head_dim is a multiple of 16 up to 256. */
+int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, int typ, const void *q, int64_t ldq,
+                             int n_heads, const void *kx, int64_t ldk, const void *v, int64_t ldv,
+                             const gb_qk_norm_params *norm, const gb_rope_params *rope, void *q_out, int64_t ldqo);
+/* Attention of the new rows (already appended): each row attends to its
+ * sequence's positions up to its own, whatever lies in the pages behind
+ * kv_lens[b]. q and out [rows][n_heads][head_dim] have the pool's type; a row
+ * that sees no position gives zeros. Table entries outside [0, n_pages) read
+ * page 0; kv_lens past the table count as the table's length. Any number of
+ * query heads per KV head; head_dim a multiple of 16 up to 128; scale > 0.
+ * Float32 statistics and sums; results do not depend on the order in which
+ * the GPU runs the parts. Scratch of a fixed size lives in `k`: the first call
+ * allocates it (so not inside a stream capture: GB_ERR_INVALID) and it never
+ * moves. Calls on one `k` must not overlap on the GPU; use a handle for each
+ * of several streams. */
+int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, const void *q, int64_t ldq,
+                            int n_heads, float scale, void *out, int64_t ldo);
+
 /* ---- sampling (added; the reference's roadmap item, ROADMAP.md:42-45) ----
  * One token from a logits vector on the device:
  *  1. the logits of every distinct id among the last repeat_last_n context

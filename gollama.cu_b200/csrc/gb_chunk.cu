@@ -37,6 +37,7 @@ struct ChunkArgs {
   float scale_log2;   // scale * log2(e): the softmax is taken in powers of two
   float *part;        // partial rows (part_slot)
   unsigned *counter;  // [CTAs], zero between launches
+  unsigned *err;      // a wait ran out (host memory)
 };
 
 // ---- the line of work --------------------------------------------------------
@@ -192,24 +193,25 @@ struct Walk {
   }
 };
 
-// The pool row of position p (in elements, for KV head h), -1 past the
+// The pool row of position p for KV head h, in units of `width` to a row, -1 past the
 // sequence's positions; a table entry outside the pool reads page 0, as the
 // decode attention does.
-GB_DEV long long pool_row(const ChunkArgs &a, const Seq &s, int b, int h, int p) {
+GB_DEV long long pool_row(const ChunkArgs &a, const Seq &s, int b, int h, int p, int width) {
   if (p >= s.cap) return -1;
   int phys = a.c.block_table[(long long)b * a.c.max_pages + p / a.c.page_size];
   if (phys < 0 || phys >= a.c.n_pages) phys = 0;
-  return (((long long)phys * a.c.n_kv + h) * a.c.page_size + p % a.c.page_size) * a.c.head_dim;
+  return (((long long)phys * a.c.n_kv + h) * a.c.page_size + p % a.c.page_size) * width;
 }
 
 // ---- partial rows ------------------------------------------------------------
 // A CTA leaves at most two pieces for others to join: the one its run begins
-// within (which = 0) and the one it begins and does not end (which = 1). Each
-// has RU rows of kMaxHD floats, then their maxima, then their sums.
-constexpr int kMaxHD = 128;
+// within (which = 0) and the one it begins and does not end (which = 1); a
+// third place (which = 2) is its own. Each has RU rows of kMaxHD floats, then
+// their maxima (of the scores in powers of two), then their sums.
+constexpr int kMaxHD = 128, kPlaces = 3;
 template <int RU>
 GB_DEV float *part_slot(const ChunkArgs &a, int cta, int which) {
-  return a.part + (size_t)(cta * 2 + which) * RU * (kMaxHD + 2);
+  return a.part + (size_t)(cta * kPlaces + which) * RU * (kMaxHD + 2);
 }
 
 GB_DEV float ex2(float x) {
@@ -264,7 +266,7 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = 0; p0 < lim; p0 += 32) {
     const int p = p0 + lane;
-    const long long at = p < lim ? pool_row(a, s, b, head, p) : -1;
+    const long long at = p < lim ? pool_row(a, s, b, head, p, hd) : -1;
     float sc = 0.f;
     if (at >= 0)
       for (int d = 0; d < hd; d += 4) {
@@ -293,44 +295,61 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
   if (4 * lane < hd) put4<T>(a.out, row * a.ldo + hq + 4 * lane, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
-// Joins the pieces of a unit, CTA by CTA: one warp to a row, four dimensions to a lane.
-template <int T, int RU, typename W>
-GB_DEV void join_pieces(const ChunkArgs &a, const W &w, int warp, int warps) {
+// Joins the pieces of a unit, CTA by CTA: one warp to a row, four dimensions
+// to a lane. With HALVES a place holds two pieces of the same rows, RU / 2
+// rows apart. `own`: the unit is this CTA's alone, in its own place.
+struct Unit {
+  Seq s;
+  int b, head, r0, nr, c_first, c_last;
+};
+template <int T, int RU, bool HALVES>
+__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int warp, int warps, bool own) {
   const int lane = threadIdx.x & 31, hd = a.c.head_dim;
+  const int c0 = own ? (int)blockIdx.x : w.c_first, c1 = own ? (int)blockIdx.x : w.c_last;
+  const int parts = HALVES ? 2 : 1, n = (c1 - c0 + 1) * parts;
   for (int r = warp; r < w.nr; r += warps) {
+    auto place = [&](int i) {
+      const int c = c0 + i / parts;
+      return part_slot<RU>(a, c, own ? 2 : c == c0);
+    };
+    auto row = [&](int i) { return r + i % parts * (RU / 2); };
     float m = -INFINITY;
-    for (int c = w.c_first + lane; c <= w.c_last; c += 32)
-      m = fmaxf(m, __ldcg(part_slot<RU>(a, c, c == w.c_first) + RU * kMaxHD + r));
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(place(i) + RU * kMaxHD + row(i)));
     m = gb_warp_max(m);
+    if (m == -INFINITY) m = 0.f;
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m > -INFINITY)
-      for (int c = w.c_first; c <= w.c_last; c++) {
-        const float *p = part_slot<RU>(a, c, c == w.c_first);
-        const float f = ex2(__ldcg(p + RU * kMaxHD + r) - m);
-        l = fmaf(f, __ldcg(p + RU * (kMaxHD + 1) + r), l);
-        const float4 v = __ldcg((const float4 *)(p + (size_t)r * kMaxHD) + lane);
-        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-      }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    if (4 * lane < hd) {
-      const int pr = w.r0 + r;
-      const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd + 4 * lane;
-      put4<T>(a.out, at, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+#pragma unroll 4
+    for (int i = 0; i < n; i++) {
+      const float *p = place(i);
+      const float mi = __ldcg(p + RU * kMaxHD + row(i)), li = __ldcg(p + RU * (kMaxHD + 1) + row(i));
+      const float4 v = __ldcg((const float4 *)(p + (size_t)row(i) * kMaxHD) + lane);
+      if (mi == -INFINITY && li == 0.f) continue;  // nothing seen there; its outputs may not have been written
+      const float f = ex2(mi - m);
+      l = fmaf(f, li, l);
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
     }
-    const bool odd = !isfinite(o.x * inv) || !isfinite(o.y * inv) || !isfinite(o.z * inv) || !isfinite(o.w * inv);
-    if (__any_sync(0xffffffffu, 4 * lane < hd && odd)) redo_row<T>(a, w.s, w.b, w.head, w.r0 + r);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int pr = w.r0 + r;
+    bool odd = false;
+    if (4 * lane < hd) {
+      const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd + 4 * lane;
+      o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+      put4<T>(a.out, at, o.x, o.y, o.z, o.w);
+      odd = !isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w);
+    }
+    if (__any_sync(0xffffffffu, odd)) redo_row<T>(a, w.s, w.b, w.head, pr);
   }
 }
 
-// ---- the kernel on CUDA cores ------------------------------------------------
+// ---- the kernel on CUDA cores (float32 pools) ------------------------------------------------
 // 64 packed rows by tiles of 64 positions, 16 x 16 threads: thread (ty, tx)
 // holds the scores of rows 4 ty.. and positions 4 tx.., and of its rows'
 // outputs the dimensions 4 tx + 64 j. Everything float32.
 constexpr int kCR = 64, kCT = 64, kCN = 256, kCS = 68;  // rows, tile, threads, padded row of the transposed tiles
 
-template <int T, int HD>
-__global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constant__ ChunkArgs a) {
+template <int HD>
+__global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_constant__ ChunkArgs a) {
   extern __shared__ __align__(16) float sm[];
   float *qs = sm;                  // [HD][kCS]: q transposed
   float *ks = qs + HD * kCS;       // [HD][kCS]: k transposed; then [kCT][kCS]: p transposed
@@ -351,7 +370,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constan
       float v[4] = {0.f, 0.f, 0.f, 0.f};
       if (r < w.nr && d < hd) {
         const int pr = w.r0 + r;
-        ld4<T>(a.q, (long long)(w.s.q0 + pr / a.G) * a.ldq + (long long)(w.head * a.G + pr % a.G) * hd + d, v);
+        ld4<GB_F32>(a.q, (long long)(w.s.q0 + pr / a.G) * a.ldq + (long long)(w.head * a.G + pr % a.G) * hd + d, v);
       }
 #pragma unroll
       for (int e = 0; e < 4; e++) qs[(d + e) * kCS + r] = v[e];
@@ -366,13 +385,13 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constan
       for (int d = 0; d < HD / 16; d++) o[r][d] = 0.f;
     }
     for (int t = w.t0; t < w.t1; t++) {
-      if (tid < kCT) prow[tid] = pool_row(a, w.s, w.b, w.head, t * kCT + tid);
+      if (tid < kCT) prow[tid] = pool_row(a, w.s, w.b, w.head, t * kCT + tid, hd);
       __syncthreads();
       for (int i = tid; i < kCT * (HD / 4); i += kCN) {
         const int p = i % kCT, d = i / kCT * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         const long long at = prow[p];
-        if (at >= 0 && d < hd) ld4<T>(a.c.k_pool, at + d, v);
+        if (at >= 0 && d < hd) ld4<GB_F32>(a.c.k_pool, at + d, v);
 #pragma unroll
         for (int e = 0; e < 4; e++) ks[(d + e) * kCS + p] = v[e];
       }
@@ -380,7 +399,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constan
         const int p = i / (HD / 4), d = i % (HD / 4) * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         const long long at = prow[p];
-        if (at >= 0 && d < hd) ld4<T>(a.c.v_pool, at + d, v);
+        if (at >= 0 && d < hd) ld4<GB_F32>(a.c.v_pool, at + d, v);
         *(float4 *)(vs + p * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
       }
       __syncthreads();
@@ -447,7 +466,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constan
       for (int r = 0; r < 4; r++) {
         const int pr = w.r0 + 4 * ty + r;
         const bool on = 4 * ty + r < w.nr;
-        const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+        const float inv = l[r] != 0.f ? 1.f / l[r] : 0.f;
         const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
         bool odd = false;
 #pragma unroll
@@ -456,13 +475,13 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constan
             float v[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] = o[r][4 * j + k] * inv, odd |= !isfinite(v[k]);
-            put4<T>(a.out, at + 64 * j + 4 * tx, v[0], v[1], v[2], v[3]);
+            put4<GB_F32>(a.out, at + 64 * j + 4 * tx, v[0], v[1], v[2], v[3]);
           }
         const unsigned any = __ballot_sync(0xffffffffu, odd);
 #pragma unroll
         for (int half = 0; half < 2; half++)
           if (any >> (16 * half) & 0xFFFFu)
-            redo_row<T>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r);
+            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r);
       }
       continue;
     }
@@ -485,24 +504,643 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_kernel(const __grid_constan
     __syncthreads();
     if (arrived != (unsigned)(w.c_last - w.c_first)) continue;
     __threadfence();
-    join_pieces<T, kCR>(a, w, tid >> 5, kCN / 32);
+    join_pieces<GB_F32, kCR, false>(a, {w.s, w.b, w.head, w.r0, w.nr, w.c_first, w.c_last}, tid >> 5, kCN / 32, false);
     if (tid == 0) a.counter[w.c_first] = 0u;  // ready for the next launch
   }
 }
 
-template <int T, int HD>
-int launch_simple(const ChunkArgs &a, int ctas, cudaStream_t st, const char *what) {
+// ---- the kernel on tensor cores (16-bit pools) --------------------------------
+// Units of 256 packed rows, tiles of 128 positions. Both products run on
+// tcgen05 (M = 128, float32 accumulators in tensor memory): S = Q K^T from
+// shared memory, then O += P V with P written over S in tensor memory.
+//
+// Two softmax groups of four warps, a row to a thread. In a unit of more than
+// 128 rows each group has 128 rows of its own and both use every tile; in a
+// smaller one (decoding) both have the same rows and take alternate tiles, and
+// their two results are joined like the pieces of two CTAs. Either way one
+// group's softmax runs while the tensor cores work for the other.
+//
+// K and V tiles come in order K0 V0 K1 V1 ... into a ring, with the 128-byte
+// swizzle that the descriptors name. Where the page size has a divisor of at
+// least 8 in common with the tile, one warp fetches them by TMA, a box of that
+// many rows to a lane, from wherever its page lies; what a box brings behind
+// the sequence's end is overwritten with zeros in V (0 NaN is NaN), and does
+// not matter in K. Other page sizes go through 16-byte asynchronous copies by
+// three warps, zeros behind the end. One thread issues all tcgen05.mma; they
+// run in the order issued, so S of the next tile may be queued behind the P V
+// that reads P in the same columns.
+//
+// The running maximum is let lag: the sums and outputs are rescaled only when
+// a tile's maximum exceeds it by more than 2^kSlack, so P stays below 2^8
+// (binary16 holds 65504) and most tiles leave O in tensor memory alone.
+//
+// The tensor cores take P in 16 bits. A unit of more than 128 rows rounds it
+// to the pool's type, as its result is rounded. Smaller units, which the
+// cache's bytes bound, have room for P in two parts, the rounded one and the
+// rounding's remainder (two products with V, in S's columns), and so none of
+// that error: few rows over few outstanding positions do not average it out.
+constexpr int kTR = 256, kTT = 128;       // rows of a unit, positions of a tile
+// 12 warps: 168 registers a thread, room for a row's 128 scores (a 13th warp would leave 128)
+constexpr int kSoftWarps = 8, kLoadWarps = 3, kMmaWarp = kSoftWarps + kLoadWarps;
+constexpr int kTN = (kMmaWarp + 1) * 32;  // threads
+constexpr float kSlack = 8.f;
+constexpr uint32_t kChunkBytes = 128 * 128;  // 128 rows of 64 elements
+constexpr int kRingBytes = 10 * kChunkBytes;
+template <int HD>
+constexpr int ring_slots() { return kRingBytes / (HD / 64 * (int)kChunkBytes); }
+template <int HD>
+constexpr int tc_smem() { return 2048 + 2 * HD / 64 * (int)kChunkBytes + kRingBytes; }
+
+struct TcShared {
+  uint64_t full[10], empty[10], landed[10], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free[2], fin;
+  Plan plan;
+  long long warp_sums[kTN / 32];
+  uint32_t tmem;
+  unsigned arrived;
+  int dead;
+};
+static_assert(sizeof(TcShared) <= 1024, "shared header");
+
+GB_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+GB_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+GB_DEV void tc_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(gb_smem_u32(bar))
+               : "memory");
+}
+// D[128 x N] (+)= A B^T, both from shared memory.
+GB_DEV void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A from tensor memory.
+GB_DEV void tc_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 columns of this warp's 32 lanes (no wait).
+GB_DEV void tc_ld32(uint32_t addr, float *v) {
+  uint32_t *r = (uint32_t *)v;
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+GB_DEV void tc_ld16(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+GB_DEV void tc_st16(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
+          r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
+GB_DEV void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+GB_DEV void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory descriptors, 128-byte swizzle, 128-byte rows in groups of
+// eight (1024 bytes). Rows along M or N with K contiguous (Q, K): the groups
+// are the stride. Rows along K with N contiguous (V): the groups are the
+// stride along K, and 64-element column chunks (kChunkBytes) the leading one.
+GB_DEV uint64_t desc_rows(uint32_t saddr, uint32_t leading) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16: float32 accumulators, A and B of type T, B with N contiguous when TB.
+template <int T>
+GB_DEV uint32_t idesc_of(int N, bool TB) {
+  const uint32_t f = T == GB_BF16 ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (TB ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// Every wait is bounded: when one runs out, or another thread's has, the CTA
+// goes on without waiting (all addresses stay within their buffers), ends, and
+// the error word tells.
+// The CTA's last waits (`last`: for copies and products in flight) are made all the same.
+GB_DEV void bar_wait(TcShared *sh, uint64_t *bar, uint32_t parity, unsigned *err, bool last = false) {
+  for (uint32_t i = 0; i < GB_WAIT_LIMIT; i++) {
+    if (gb_mbar_try_wait(bar, parity)) return;
+    if (!last && (i & 63) == 63 && *(volatile int *)&sh->dead) return;
+  }
+  *(volatile int *)&sh->dead = 1;
+  *(volatile unsigned *)err = GB_DEVERR_TIMEOUT;
+}
+
+GB_DEV void cp_async16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+GB_DEV void cp_async_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(gb_smem_u32(bar)) : "memory");
+}
+
+// A warp's copies of its 32 rows of a tile: `at` is the lane's row (elements
+// from base, -1: zeros), ppr 16-byte pieces a row, several rows a pass.
+GB_DEV void load_rows(const uint16_t *base, long long at, uint32_t tile, int row0, int ppr, int lane) {
+  const int rpp = 32 / ppr, sub = lane / ppr, pc = lane - sub * ppr;
+  const uint32_t chunk = tile + (uint32_t)(pc >> 3) * kChunkBytes;
+#pragma unroll 8
+  for (int r0 = 0; r0 < 32; r0 += rpp) {
+    const int r = r0 + sub;
+    const long long from = __shfl_sync(0xffffffffu, at, r & 31);
+    if (sub < rpp && r < 32) {
+      const int row = row0 + r;
+      cp_async16(chunk + row * 128 + ((pc ^ row) & 7) * 16, base + (from < 0 ? 0 : from) + pc * 8, from >= 0);
+    }
+  }
+}
+
+// A unit's queries, 32 rows at a time in turn by `warps` warps; zeros past its rows.
+GB_DEV void load_q(const ChunkArgs &a, const Seq &s, int u0, int nr, int head, uint32_t q_at, uint32_t tile, int lw,
+                   int warps, int ppr, int lane) {
+  for (int j = lw; j < (nr > 128 ? 8 : 4); j += warps) {
+    const int r = j * 32 + lane, pr = u0 + r;
+    const long long at =
+        r < nr ? (long long)(s.q0 + pr / a.G) * a.ldq + (long long)(head * a.G + pr % a.G) * a.c.head_dim : -1;
+    load_rows((const uint16_t *)a.q, at, q_at + (j >> 2) * tile, (j & 3) * 32, ppr, lane);
+  }
+}
+
+template <int T>
+GB_DEV uint32_t pack2(float x, float y) {
+  if constexpr (T == GB_F16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const uint32_t *)&h;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t *)&h;
+  }
+}
+
+// The rows a TMA box holds: the page size's common divisor with a tile.
+__host__ GB_DEV int box_rows(int page_size) {
+  const int low = page_size & -page_size;
+  return low < kTT ? low : kTT;
+}
+
+GB_DEV void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(gb_smem_u32(bar))
+      : "memory");
+}
+
+// What a packed pair leaves of (x, y): the remainder, exact in float32.
+template <int T>
+GB_DEV uint32_t pack2_rest(float x, float y, uint32_t p) {
+  if constexpr (T == GB_F16) {
+    const float2 f = __half22float2(*(const __half2 *)&p);
+    return pack2<T>(x - f.x, y - f.y);
+  } else {
+    return pack2<T>(x - __uint_as_float(p << 16), y - __uint_as_float(p & 0xFFFF0000u));
+  }
+}
+
+template <int T, int HD, bool TMA>
+__global__ void __launch_bounds__(kTN, 1)
+    attn_chunk_tc_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map) {
+  extern __shared__ uint8_t raw[];
+  uint8_t *const base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  TcShared *const sh = (TcShared *)base;
+  const uint32_t q_at = gb_smem_u32(base) + 1024;
+  constexpr uint32_t kTile = HD / 64 * kChunkBytes;
+  constexpr int NS = ring_slots<HD>();
+  const uint32_t ring = q_at + 2 * kTile;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.c.head_dim;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) gb_mbar_init(&sh->full[i], TMA ? 1 : kLoadWarps * 32), gb_mbar_init(&sh->empty[i], 1), gb_mbar_init(&sh->landed[i], 1);
+    gb_mbar_init(&sh->q_full, (TMA ? 2 : kLoadWarps) * 32);
+    gb_mbar_init(&sh->q_empty, 1);
+    for (int g = 0; g < 2; g++) {
+      gb_mbar_init(&sh->s_full[g], 1);
+      gb_mbar_init(&sh->p_full[g], 4);
+      gb_mbar_init(&sh->pv_done[g], 1);
+      gb_mbar_init(&sh->o_free[g], 4);
+    }
+    gb_mbar_init(&sh->fin, 1);
+    sh->dead = 0;
+    gb_mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gb_smem_u32(&sh->tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  make_plan<kTR, kTT, kTN>(a, &sh->plan, sh->warp_sums);
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+  Walk<kTR, kTT> w;
+  w.start(a, sh->plan);
+
+  if (TMA && warp == kSoftWarps) {
+    // ---- K and V by TMA: lane = (box of rows, 64-element column chunk)
+    const int br = box_rows(a.c.page_size), nbox = kTT / br, chunks = (hd + 63) / 64;
+    const int box = lane % nbox, chunk = lane / nbox;
+    uint32_t n = 0;
+    while (w.next(a)) {
+      // the box's first row in the pool (rows of head_dim), for tile t
+      auto first_row = [&](int t) {
+        const int p = t * kTT + box * br;
+        return t < w.t1 && chunk < chunks ? pool_row(a, w.s, w.b, w.head, p, 1) : -1;
+      };
+      long long at = first_row(w.t0);
+      for (int t = w.t0; t < w.t1; t++) {
+        const long long ahead = first_row(t + 1);  // its table entry is on its way meanwhile
+        const int held = min(max(w.s.cap - t * kTT, 0), kTT), boxes = (held + br - 1) / br;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++, n++) {
+          const uint32_t slot = n % NS;
+          bar_wait(sh, &sh->empty[slot], (n / NS & 1) ^ 1, a.err);
+          // V at the sequence's end goes through the warp that puts the zeros, which then reports it full
+          uint64_t *bar = kv && held < kTT ? &sh->landed[slot] : &sh->full[slot];
+          if (lane == 0) gb_mbar_expect_tx(bar, (uint32_t)(boxes * chunks * br) * 128);
+          __syncwarp();
+          if (at >= 0)
+            tma_box(ring + slot * kTile + chunk * kChunkBytes + box * br * 128, kv ? &v_map : &k_map, chunk * 64, (int)at,
+                    bar);
+        }
+        at = ahead;
+      }
+    }
+    // whatever was fetched has landed before the CTA ends
+    for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) bar_wait(sh, &sh->full[i % NS], i / NS & 1, a.err, true);
+  } else if (TMA && warp < kMmaWarp && warp > kSoftWarps) {
+    // ---- queries (two warps), and zeros over V behind the sequence's end (one of them)
+    const int lw = warp - kSoftWarps - 1, ppr = hd / 8;
+    uint32_t n0 = 0, pieces = 0, phase = 0;  // bit i: parity of the next landing in slot i
+    while (w.next(a)) {
+      bar_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err);
+      load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, lw, 2, ppr, lane);
+      cp_async_arrive(&sh->q_full);
+      pieces++;
+      const int last = w.s.cap / kTT;  // the tile that the end lies in
+      if (lw == 0 && last >= w.t0 && last < w.t1) {
+        const uint32_t slot = (n0 + 2 * (last - w.t0) + 1) % NS;
+        bar_wait(sh, &sh->landed[slot], phase >> slot & 1, a.err);
+        phase ^= 1u << slot;
+        for (int i = (w.s.cap % kTT) * 8 + lane; i < kTT * 8; i += 32)
+          for (int c = 0; c < HD / 64; c++)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + slot * kTile + c * kChunkBytes + i * 16),
+                         "r"(0)
+                         : "memory");
+        gb_fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) gb_mbar_arrive(&sh->full[slot]);
+      }
+      n0 += 2 * (w.t1 - w.t0);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (!TMA && warp >= kSoftWarps && warp < kMmaWarp) {
+    // ---- queries, K and V by asynchronous copies
+    // A tile's four blocks of 32 rows go round the three warps, one block on with each tile.
+    const int lw = warp - kSoftWarps, ppr = hd / 8;
+    uint32_t n = 0, pieces = 0;
+    auto block = [&](int t, int k) { return (lw + 3 - t % 3) % 3 + 3 * k; };  // k = 0, 1; 4 and on: none
+    auto row_of = [&](int t, int k) {
+      const int j = block(t, k);
+      return t < w.t1 && j < 4 ? pool_row(a, w.s, w.b, w.head, t * kTT + j * 32 + lane, hd) : -1;
+    };
+    while (w.next(a)) {
+      bar_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err);
+      load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, lw, kLoadWarps, ppr, lane);
+      cp_async_arrive(&sh->q_full);
+      pieces++;
+      long long at0 = row_of(w.t0, 0), at1 = row_of(w.t0, 1);
+      for (int t = w.t0; t < w.t1; t++) {
+        // the next tile's table entries are on their way while this one's rows are
+        const long long ahead0 = row_of(t + 1, 0), ahead1 = row_of(t + 1, 1);
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++, n++) {
+          const uint32_t slot = n % NS;
+          bar_wait(sh, &sh->empty[slot], (n / NS & 1) ^ 1, a.err);
+          const uint16_t *pool = (const uint16_t *)(kv ? a.c.v_pool : a.c.k_pool);
+          load_rows(pool, at0, ring + slot * kTile, block(t, 0) * 32, ppr, lane);
+          if (block(t, 1) < 4) load_rows(pool, at1, ring + slot * kTile, block(t, 1) * 32, ppr, lane);
+          cp_async_arrive(&sh->full[slot]);
+        }
+        at0 = ahead0, at1 = ahead1;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kMmaWarp) {
+    // ---- the one thread that issues the products
+    if (lane == 0) {
+      const uint32_t iq = idesc_of<T>(kTT, false), iv = idesc_of<T>(hd, true);
+      // ring position of the piece, pieces, P's taken of each group
+      uint32_t n0 = 0, pieces = 0, np[2] = {0, 0};
+      auto qk = [&](int g, int qt, uint32_t n) {     // S_g = Q_qt K^T, K at ring position n
+        const uint32_t k_at = ring + n % NS * kTile;
+        for (int kk = 0; kk < hd / 16; kk++) {
+          const uint32_t off = (uint32_t)(kk >> 2) * kChunkBytes + (uint32_t)(kk & 3) * 32;
+          tc_mma(tmem + g * 128, desc_rows(q_at + qt * kTile + off, 16), desc_rows(k_at + off, 16), iq, kk != 0);
+        }
+        tc_commit(&sh->s_full[g]);
+      };
+      auto pv = [&](int g, uint32_t n, bool first, int parts) {  // O_g (+)= P_g V, V at ring position n
+        const uint32_t v_at = ring + n % NS * kTile;
+        for (int kk = 0; kk < parts * (kTT / 16); kk++)
+          tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + kk * 8, desc_rows(v_at + (kk & 7) * 2048, kChunkBytes), iv,
+                    !first || kk != 0);
+        tc_commit(&sh->pv_done[g]);
+      };
+      auto loaded = [&](uint32_t n) {
+        bar_wait(sh, &sh->full[n % NS], n / NS & 1, a.err);
+        gb_fence_proxy_async();  // the copies' bytes, seen here, before the tensor cores read them
+      };
+      auto p_ready = [&](int g) {
+        bar_wait(sh, &sh->p_full[g], np[g]++ & 1, a.err);
+        tc_fence_after();
+      };
+      while (w.next(a)) {
+        const int n = w.t1 - w.t0;
+        const bool both = w.nr > 128;  // both groups use each tile
+        bar_wait(sh, &sh->q_full, pieces & 1, a.err);
+        gb_fence_proxy_async();
+        for (int t = 0; t < (both ? 1 : min(n, 2)); t++) {
+          loaded(n0 + 2 * t);
+          if (both) qk(0, 0, n0), qk(1, 1, n0);
+          else qk(t, 0, n0 + 2 * t);
+          tc_commit(&sh->empty[(n0 + 2 * t) % NS]);
+        }
+        if (both ? n == 1 : n <= 2) tc_commit(&sh->q_empty);
+        // O of the last unit has been read: at a group's first P V of this one
+        const uint32_t free_parity = (pieces & 1) ^ 1;
+        for (int t = 0; t < n; t++) {
+          const uint32_t v = n0 + 2 * t + 1;
+          loaded(v);
+          if (both) {
+            const uint32_t k = v + 1;
+            for (int g = 0; g < 2; g++) {
+              if (t == 0) bar_wait(sh, &sh->o_free[g], free_parity, a.err);
+              p_ready(g);
+              pv(g, v, t == 0, 1);
+              if (g) tc_commit(&sh->empty[v % NS]);
+              if (t + 1 < n) {
+                if (!g) loaded(k);
+                qk(g, g, k);
+                if (g) tc_commit(&sh->empty[k % NS]);
+              }
+            }
+            if (t + 2 == n) tc_commit(&sh->q_empty);
+          } else {
+            const int g = t & 1;
+            if (t < 2) bar_wait(sh, &sh->o_free[g], free_parity, a.err);
+            p_ready(g);
+            pv(g, v, t < 2, 2);
+            tc_commit(&sh->empty[v % NS]);
+            if (t + 2 < n) {
+              const uint32_t k = n0 + 2 * (t + 2);
+              loaded(k);
+              qk(g, 0, k);
+              tc_commit(&sh->empty[k % NS]);
+              if (t + 3 == n) tc_commit(&sh->q_empty);
+            }
+          }
+        }
+        n0 += 2 * n;
+        pieces++;
+      }
+      // nothing is in flight when the tensor memory is given back
+      tc_commit(&sh->fin);
+      bar_wait(sh, &sh->fin, 0, a.err, true);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread = row
+    const int g = warp >> 2, row = tid & 127;
+    const uint32_t s_at = tmem + g * 128 + ((uint32_t)(warp & 3) << 21), o_at = s_at + 256;
+    uint32_t ns = 0;  // tiles this group has taken
+    while (w.next(a)) {
+      const bool both = w.nr > 128;
+      const int ur = (both ? g * 128 : 0) + row, pr = w.r0 + ur;
+      const bool mine = ur < w.nr;
+      const bool warp_on = ur - lane < w.nr;
+      // rows past the unit's are computed with zero queries and not looked at
+      const int lim = mine ? visible(w.s, a.G, pr) : 0x7FFFFFFF;
+      float m = -INFINITY, l = 0.f;
+      int done = 0;
+      for (int t = w.t0 + (both ? 0 : g); t < w.t1; t += both ? 1 : 2, ns++, done++) {
+        bar_wait(sh, &sh->s_full[g], ns & 1, a.err);
+        tc_fence_after();
+        if (warp_on) {
+          float s[128];
+#pragma unroll
+          for (int c = 0; c < 4; c++) tc_ld32(s_at + 32 * c, s + 32 * c);
+          tc_wait_ld();
+          const int rel = lim - t * kTT;
+          if (__any_sync(0xffffffffu, rel < kTT)) {
+#pragma unroll
+            for (int c = 0; c < 128; c++) s[c] = c < rel ? s[c] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          const bool raise = top > m + kSlack || m == -INFINITY;
+          const float mn = raise ? fmaxf(m, top) : m;
+          if (__any_sync(0xffffffffu, raise)) {
+            const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+            l *= f;
+            if (done) {  // O is there: the last P V must have ended before it is scaled
+              bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
+              tc_fence_after();
+              for (int c = 0; c < hd; c += 16) {
+                uint32_t o[16];
+                tc_ld16(o_at + c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc_st16(o_at + c, o);
+              }
+            }
+          }
+          m = mn;
+          const float ms = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 4; h++) {
+            uint32_t p[16], rest[16];
+#pragma unroll
+            for (int c = 0; c < 16; c++) {
+              const float x = ex2(fmaf(s[32 * h + 2 * c], a.scale_log2, -ms));
+              const float y = ex2(fmaf(s[32 * h + 2 * c + 1], a.scale_log2, -ms));
+              sum[2 * (c & 1)] += x;
+              sum[2 * (c & 1) + 1] += y;
+              p[c] = pack2<T>(x, y);
+              if (!both) rest[c] = pack2_rest<T>(x, y, p[c]);
+            }
+            tc_st16(s_at + 16 * h, p);
+            if (!both) tc_st16(s_at + 64 + 16 * h, rest);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tc_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) gb_mbar_arrive(&sh->p_full[g]);
+      }
+      // ---- the unit's end: its rows out of tensor memory
+      const bool whole = w.t0 == 0 && w.t1 == w.nt;
+      if (done) {
+        bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
+        tc_fence_after();
+      }
+      if (whole && both) {
+        bool odd = false;
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
+        if (warp_on)
+          for (int c = 0; c < hd; c += 32) {
+            float o[32];
+            tc_ld32(o_at + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              if (mine && c + e < hd) {
+                uint32_t u[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  const float x = o[e + 2 * k] * inv, y = o[e + 2 * k + 1] * inv;
+                  odd |= !isfinite(x) || !isfinite(y);
+                  u[k] = pack2<T>(x, y);
+                }
+                *(uint4 *)((uint16_t *)a.out + at + c + e) = make_uint4(u[0], u[1], u[2], u[3]);
+              }
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) gb_mbar_arrive(&sh->o_free[g]);
+        for (unsigned any = __ballot_sync(0xffffffffu, odd); any; any &= any - 1)
+          redo_row<T>(a, w.s, w.b, w.head, pr - lane + __ffs(any) - 1);
+        continue;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the CTA's own place has been read out
+      float *const dst = part_slot<kTR>(a, blockIdx.x, whole ? 2 : w.t0 == 0);
+      const int at = g * 128 + row;  // groups with the same rows leave two results
+      if (warp_on && done)
+        for (int c = 0; c < hd; c += 32) {
+          float o[32];
+          tc_ld32(o_at + c, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (mine && c + e < hd)
+              *(float4 *)(dst + (size_t)at * kMaxHD + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      if (mine) {
+        dst[kTR * kMaxHD + at] = m;
+        dst[kTR * (kMaxHD + 1) + at] = l;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) gb_mbar_arrive(&sh->o_free[g]);
+      __threadfence();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (!whole) {
+        if (tid == 0) sh->arrived = atomicAdd(a.counter + w.c_first, 1u);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (sh->arrived != (unsigned)(w.c_last - w.c_first)) continue;
+        __threadfence();
+      }
+      const Unit unit = {w.s, w.b, w.head, w.r0, w.nr, w.c_first, w.c_last};
+      if (both) join_pieces<T, kTR, false>(a, unit, warp, kSoftWarps, whole);
+      else join_pieces<T, kTR, true>(a, unit, warp, kSoftWarps, whole);
+      if (!whole && tid == 0) a.counter[w.c_first] = 0u;  // ready for the next launch
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A pool as rows of head_dim 16-bit elements, in boxes of 64 columns by `br`
+// rows (zeros past head_dim).
+int pool_map(const ChunkArgs &a, void *pool, int br, CUtensorMap *map, const char *what) {
+  static EncodeTiledFn encode = nullptr;
+  if (!encode) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess || !fn)
+      return gb_fail(GB_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
+    encode = (EncodeTiledFn)fn;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.c.n_pages * a.c.n_kv * a.c.page_size};
+  const cuuint64_t strides[1] = {(cuuint64_t)a.c.head_dim * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)br}, one[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, pool, dims, strides, box, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return gb_fail(GB_ERR_CUDA, "%s: tensor map encode failed (%d)", what, (int)r);
+  return GB_OK;
+}
+
+template <int T, int HD, bool TMA>
+int launch_tc(const ChunkArgs &a, int sms, cudaStream_t st, const char *what) {
+  CUtensorMap k_map = {}, v_map = {};
+  if (TMA) {
+    const int br = box_rows(a.c.page_size);
+    int rc = pool_map(a, a.c.k_pool, br, &k_map, what);
+    if (rc == GB_OK) rc = pool_map(a, a.c.v_pool, br, &v_map, what);
+    if (rc != GB_OK) return rc;
+  }
+  GB_CUDA(cudaFuncSetAttribute(attn_chunk_tc_kernel<T, HD, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               tc_smem<HD>()),
+          what);
+  attn_chunk_tc_kernel<T, HD, TMA><<<(unsigned)sms, kTN, tc_smem<HD>(), st>>>(a, k_map, v_map);
+  GB_CUDA(cudaGetLastError(), what);
+  return GB_OK;
+}
+
+template <int T>
+int launch_16(const ChunkArgs &a, int sms, cudaStream_t st, const char *what) {
+  // a box starts on a group of eight swizzled rows, and its row is a 32-bit coordinate
+  const bool tma = box_rows(a.c.page_size) >= 8 && (long long)a.c.n_pages * a.c.n_kv * a.c.page_size < (1LL << 31);
+  if (a.c.head_dim <= 64) return tma ? launch_tc<T, 64, true>(a, sms, st, what) : launch_tc<T, 64, false>(a, sms, st, what);
+  return tma ? launch_tc<T, 128, true>(a, sms, st, what) : launch_tc<T, 128, false>(a, sms, st, what);
+}
+
+template <int HD>
+int launch_f32(const ChunkArgs &a, int ctas, cudaStream_t st, const char *what) {
   const int smem = (2 * HD * kCS + kCT * HD) * (int)sizeof(float);
-  GB_CUDA(cudaFuncSetAttribute(attn_chunk_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
-  attn_chunk_kernel<T, HD><<<(unsigned)ctas, kCN, smem, st>>>(a);
+  GB_CUDA(cudaFuncSetAttribute(attn_chunk_f32_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
+  attn_chunk_f32_kernel<HD><<<(unsigned)ctas, kCN, smem, st>>>(a);
   GB_CUDA(cudaGetLastError(), what);
   return GB_OK;
 }
 
 }  // namespace
 
-// Floats of partial rows and number of counters of a launch on `sms` SMs (two CTAs an SM).
-size_t gb_attn_chunk_part_floats(int sms) { return (size_t)sms * 2 * 2 * kCR * (kMaxHD + 2); }
+// Floats of partial rows and number of counters of a launch on `sms` SMs: two
+// CTAs an SM in float32, one on the tensor cores.
+size_t gb_attn_chunk_part_floats(int sms) {
+  return (size_t)sms * kPlaces * std::max(2 * kCR, kTR) * (kMaxHD + 2);
+}
 int gb_attn_chunk_counters(int sms) { return 2 * sms; }
 
 int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale,
@@ -529,19 +1167,18 @@ int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, i
 }
 
 int gb_attn_chunk_launch(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale, void *out,
-                         long long ldo, float *part, unsigned *counter, int sms, cudaStream_t st) {
+                         long long ldo, float *part, unsigned *counter, unsigned *err, int sms,
+                         cudaStream_t st) {
   const char *what = "gpu: chunk attention";
   ChunkArgs a = {};
   a.c = *c;
   a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
   a.n_heads = n_heads, a.G = n_heads / c->n_kv;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  a.part = part, a.counter = counter;
-#define GB_CHUNK(T) \
-  if (c->kv_typ == T) return c->head_dim <= 64 ? launch_simple<T, 64>(a, 2 * sms, st, what) : launch_simple<T, 128>(a, 2 * sms, st, what);
-  GB_CHUNK(GB_F32)
-  GB_CHUNK(GB_F16)
-  GB_CHUNK(GB_BF16)
-#undef GB_CHUNK
+  a.part = part, a.counter = counter, a.err = err;
+  if (c->kv_typ == GB_F32)
+    return c->head_dim <= 64 ? launch_f32<64>(a, 2 * sms, st, what) : launch_f32<128>(a, 2 * sms, st, what);
+  if (c->kv_typ == GB_F16) return launch_16<GB_F16>(a, sms, st, what);
+  if (c->kv_typ == GB_BF16) return launch_16<GB_BF16>(a, sms, st, what);
   return gb_fail(GB_ERR_UNSUPPORTED, "%s: pool type %d", what, c->kv_typ);
 }

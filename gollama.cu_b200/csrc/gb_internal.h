@@ -253,7 +253,8 @@ int gb_attn_chunk_counters(int sms);
 int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale,
                         const void *out, long long ldo);
 int gb_attn_chunk_launch(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale, void *out,
-                         long long ldo, float *part, unsigned *counter, int sms, cudaStream_t st);
+                         long long ldo, float *part, unsigned *counter, unsigned *err, int sms,
+                         cudaStream_t st);
 
 // gb_sample.cu: one token from logits[n]; parameters by value (p_host) or
 // from device memory (p_dev, for graph replays); the penalty window is

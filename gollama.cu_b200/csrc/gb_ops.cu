@@ -498,6 +498,7 @@ struct gb_kernels {
   unsigned *pws_counter = nullptr;
   size_t pws_counters = 0;
   float *cws = nullptr;  // chunk attention: partial rows + counters, one allocation of a fixed size
+  unsigned *cerr = nullptr;  // its error word, in page-locked host memory the kernel writes to
   int sms = 0;
 };
 
@@ -551,6 +552,7 @@ int gb_gpu_close(gb_kernels *k) {
   if (k->pws) cudaFree(k->pws);
   if (k->pws_counter) cudaFree(k->pws_counter);
   if (k->cws) cudaFree(k->cws);
+  if (k->cerr) cudaFreeHost(k->cerr);
   if (k->status) cudaFree(k->status);
   delete k;
   return GB_OK;
@@ -999,6 +1001,10 @@ int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c
   if (!c->rows || !c->batch) return GB_OK;
   const OnDevice on(k);
   const cudaStream_t st = (cudaStream_t)stream;
+  if (k->cerr && *(volatile unsigned *)k->cerr) {
+    *k->cerr = 0;
+    return gb_fail(GB_ERR_TIMEOUT, "gpu: chunk attention: a wait in an earlier call ran out; its results are not valid");
+  }
   const size_t floats = gb_attn_chunk_part_floats(k->sms);
   if (!k->cws) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -1006,6 +1012,10 @@ int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c
     if (cap != cudaStreamCaptureStatusNone)
       return gb_fail(GB_ERR_INVALID, "gpu: chunk attention: the handle's first call allocates: make it before a capture");
     const size_t counters = (size_t)gb_attn_chunk_counters(k->sms) * sizeof(unsigned);
+    if (!k->cerr) {
+      GB_CUDA(cudaHostAlloc(&k->cerr, sizeof(unsigned), cudaHostAllocMapped), "gpu: chunk attention: workspace");
+      *k->cerr = 0;
+    }
     float *ws = nullptr;
     GB_CUDA(cudaMalloc(&ws, floats * sizeof(float) + counters), "gpu: chunk attention: workspace");
     // counters zero before this call's launch, and before any other stream's
@@ -1017,7 +1027,8 @@ int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c
     }
     k->cws = ws;
   }
-  return gb_attn_chunk_launch(c, q, ldq, n_heads, scale, out, ldo, k->cws, (unsigned *)(k->cws + floats), k->sms, st);
+  return gb_attn_chunk_launch(c, q, ldq, n_heads, scale, out, ldo, k->cws, (unsigned *)(k->cws + floats),
+                              k->cerr, k->sms, st);
 }
 
 // model.Argmax, model/model.go:376.

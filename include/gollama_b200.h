@@ -240,7 +240,9 @@ int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *
  * the GPU runs the parts. Scratch of a fixed size lives in `k`: the first call
  * allocates it (so not inside a stream capture: GB_ERR_INVALID) and it never
  * moves. Calls on one `k` must not overlap on the GPU; use a handle for each
- * of several streams. */
+ * of several streams. The kernel's waits are bounded: should one run out, the
+ * call ends with undefined outputs and the handle's next call of this function
+ * returns GB_ERR_TIMEOUT. */
 int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, const void *q, int64_t ldq,
                             int n_heads, float scale, void *out, int64_t ldo);
 

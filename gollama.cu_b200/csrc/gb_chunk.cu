@@ -583,24 +583,52 @@ GB_DEV void tc_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 32 columns of this warp's 32 lanes (no wait).
-GB_DEV void tc_ld32(uint32_t addr, float *v) {
-  uint32_t *r = (uint32_t *)v;
+// Columns of this warp's 32 lanes into registers. The wait is part of the same
+// statement: the loads are asynchronous, and between them and a wait of its own
+// the compiler may move the results, or give their registers to other values.
+GB_DEV void tc_ld16(uint32_t addr, uint32_t *v) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16]; "
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr)
+      : "memory");
 }
-GB_DEV void tc_ld16(uint32_t addr, uint32_t *r) {
+GB_DEV void tc_ld32(uint32_t addr, uint32_t *v) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32]; "
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+        "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+        "=r"(v[30]), "=r"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+GB_DEV void tc_ld64(uint32_t addr, uint32_t *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%64]; "
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,"
+      "%60,%61,%62,%63}, [%65]; "
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+        "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+        "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]),
+        "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]),
+        "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]), "=r"(v[50]),
+        "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]), "=r"(v[57]),
+        "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+      : "r"(addr), "r"(addr + 32)
+      : "memory");
 }
 GB_DEV void tc_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
@@ -610,7 +638,6 @@ GB_DEV void tc_st16(uint32_t addr, const uint32_t *r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
-GB_DEV void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 GB_DEV void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory descriptors, 128-byte swizzle, 128-byte rows in groups of
@@ -618,9 +645,13 @@ GB_DEV void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "me
 // are the stride. Rows along K with N contiguous (V): the groups are the
 // stride along K, and 64-element column chunks (kChunkBytes) the leading one.
 GB_DEV uint64_t desc_rows(uint32_t saddr, uint32_t leading) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+  const uint32_t lo = (saddr >> 4 & 0x3FFFu) | (leading >> 4 << 16);
+  return (uint64_t)((1024u >> 4) | 1u << 14 | 2u << 29) << 32 | lo;
 }
+// Where P's 16 positions 16 k.. lie among S's columns: the 32 columns of
+// scores 32 h.. hold their P (16 columns), then its remainder, so that no
+// score is overwritten before it is read.
+GB_DEV constexpr int p_column(int k) { return 32 * (k >> 1) + 8 * (k & 1); }
 // kind::f16: float32 accumulators, A and B of type T, B with N contiguous when TB.
 template <int T>
 GB_DEV uint32_t idesc_of(int N, bool TB) {
@@ -841,88 +872,104 @@ __global__ void __launch_bounds__(kTN, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kMmaWarp) {
-    // ---- the one thread that issues the products
-    if (lane == 0) {
-      const uint32_t iq = idesc_of<T>(kTT, false), iv = idesc_of<T>(hd, true);
-      // ring position of the piece, pieces, P's taken of each group
-      uint32_t n0 = 0, pieces = 0, np[2] = {0, 0};
-      auto qk = [&](int g, int qt, uint32_t n) {     // S_g = Q_qt K^T, K at ring position n
-        const uint32_t k_at = ring + n % NS * kTile;
-        for (int kk = 0; kk < hd / 16; kk++) {
+    // ---- the products: the warp walks and waits together, one elected lane issues
+    uint32_t leader;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
+    const uint32_t iq = idesc_of<T>(kTT, false), iv = idesc_of<T>(hd, true);
+    uint32_t n0 = 0, pieces = 0, np0 = 0, np1 = 0;  // ring position of the piece, pieces, P's taken of each group
+    // S_g = Q_qt K^T, K at ring position n; `k_done`: its slot's last use; `q_done`: the queries' last use
+    auto qk = [&](int g, int qt, uint32_t n, bool k_done, bool q_done) {
+      const uint32_t k_at = ring + n % NS * kTile, x_at = q_at + qt * kTile;
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
           const uint32_t off = (uint32_t)(kk >> 2) * kChunkBytes + (uint32_t)(kk & 3) * 32;
-          tc_mma(tmem + g * 128, desc_rows(q_at + qt * kTile + off, 16), desc_rows(k_at + off, 16), iq, kk != 0);
+          if (16 * kk < hd) tc_mma(tmem + g * 128, desc_rows(x_at + off, 16), desc_rows(k_at + off, 16), iq, kk != 0);
         }
         tc_commit(&sh->s_full[g]);
-      };
-      auto pv = [&](int g, uint32_t n, bool first, int parts) {  // O_g (+)= P_g V, V at ring position n
-        const uint32_t v_at = ring + n % NS * kTile;
-        for (int kk = 0; kk < parts * (kTT / 16); kk++)
-          tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + kk * 8, desc_rows(v_at + (kk & 7) * 2048, kChunkBytes), iv,
+        if (k_done) tc_commit(&sh->empty[n % NS]);
+        if (q_done) tc_commit(&sh->q_empty);
+      }
+      __syncwarp();
+    };
+    // O_g (+)= P_g V, V at ring position n
+    auto pv = [&](int g, uint32_t n, bool first, bool both, bool v_done) {
+      const uint32_t v_at = ring + n % NS * kTile;
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < kTT / 16; kk++)
+          tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + p_column(kk), desc_rows(v_at + kk * 2048, kChunkBytes), iv,
                     !first || kk != 0);
+        if (!both)
+#pragma unroll
+          for (int kk = 0; kk < kTT / 16; kk++)
+            tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + p_column(kk) + 16, desc_rows(v_at + kk * 2048, kChunkBytes),
+                      iv, 1);
         tc_commit(&sh->pv_done[g]);
-      };
-      auto loaded = [&](uint32_t n) {
-        bar_wait(sh, &sh->full[n % NS], n / NS & 1, a.err);
-        gb_fence_proxy_async();  // the copies' bytes, seen here, before the tensor cores read them
-      };
-      auto p_ready = [&](int g) {
-        bar_wait(sh, &sh->p_full[g], np[g]++ & 1, a.err);
-        tc_fence_after();
-      };
-      while (w.next(a)) {
-        const int n = w.t1 - w.t0;
-        const bool both = w.nr > 128;  // both groups use each tile
-        bar_wait(sh, &sh->q_full, pieces & 1, a.err);
-        gb_fence_proxy_async();
-        for (int t = 0; t < (both ? 1 : min(n, 2)); t++) {
-          loaded(n0 + 2 * t);
-          if (both) qk(0, 0, n0), qk(1, 1, n0);
-          else qk(t, 0, n0 + 2 * t);
-          tc_commit(&sh->empty[(n0 + 2 * t) % NS]);
+        if (v_done) tc_commit(&sh->empty[n % NS]);
+      }
+      __syncwarp();
+    };
+    auto loaded = [&](uint32_t n) {
+      bar_wait(sh, &sh->full[n % NS], n / NS & 1, a.err);
+      // the asynchronous copies' bytes, seen here, before the tensor cores read them (about 400 cycles)
+      if (!TMA) gb_fence_proxy_async();
+    };
+    auto p_ready = [&](int g) {
+      bar_wait(sh, &sh->p_full[g], (g ? np1++ : np0++) & 1, a.err);
+      tc_fence_after();
+    };
+    while (w.next(a)) {
+      const int n = w.t1 - w.t0;
+      const bool both = w.nr > 128;  // both groups use each tile
+      bar_wait(sh, &sh->q_full, pieces & 1, a.err);
+      gb_fence_proxy_async();
+      loaded(n0);
+      if (both) {
+        qk(0, 0, n0, false, false);
+        qk(1, 1, n0, true, n == 1);
+      } else {
+        qk(0, 0, n0, true, n == 1);
+        if (n > 1) {
+          loaded(n0 + 2);
+          qk(1, 0, n0 + 2, true, n == 2);
         }
-        if (both ? n == 1 : n <= 2) tc_commit(&sh->q_empty);
-        // O of the last unit has been read: at a group's first P V of this one
-        const uint32_t free_parity = (pieces & 1) ^ 1;
-        for (int t = 0; t < n; t++) {
-          const uint32_t v = n0 + 2 * t + 1;
-          loaded(v);
-          if (both) {
-            const uint32_t k = v + 1;
-            for (int g = 0; g < 2; g++) {
-              if (t == 0) bar_wait(sh, &sh->o_free[g], free_parity, a.err);
-              p_ready(g);
-              pv(g, v, t == 0, 1);
-              if (g) tc_commit(&sh->empty[v % NS]);
-              if (t + 1 < n) {
-                if (!g) loaded(k);
-                qk(g, g, k);
-                if (g) tc_commit(&sh->empty[k % NS]);
-              }
-            }
-            if (t + 2 == n) tc_commit(&sh->q_empty);
-          } else {
-            const int g = t & 1;
-            if (t < 2) bar_wait(sh, &sh->o_free[g], free_parity, a.err);
-            p_ready(g);
-            pv(g, v, t < 2, 2);
-            tc_commit(&sh->empty[v % NS]);
-            if (t + 2 < n) {
-              const uint32_t k = n0 + 2 * (t + 2);
-              loaded(k);
-              qk(g, 0, k);
-              tc_commit(&sh->empty[k % NS]);
-              if (t + 3 == n) tc_commit(&sh->q_empty);
-            }
+      }
+      // O of the last unit has been read: at a group's first P V of this one
+      const uint32_t free_parity = (pieces & 1) ^ 1;
+      for (int t = 0; t < n; t++) {
+        const uint32_t v = n0 + 2 * t + 1;
+        loaded(v);
+        if (both) {
+          if (t == 0) bar_wait(sh, &sh->o_free[0], free_parity, a.err);
+          p_ready(0);
+          pv(0, v, t == 0, true, false);
+          if (t + 1 < n) {
+            loaded(v + 1);
+            qk(0, 0, v + 1, false, false);
+          }
+          if (t == 0) bar_wait(sh, &sh->o_free[1], free_parity, a.err);
+          p_ready(1);
+          pv(1, v, t == 0, true, true);
+          if (t + 1 < n) qk(1, 1, v + 1, true, t + 2 == n);
+        } else {
+          const int g = t & 1;
+          if (t < 2) bar_wait(sh, &sh->o_free[g], free_parity, a.err);
+          p_ready(g);
+          pv(g, v, t < 2, false, true);
+          if (t + 2 < n) {
+            loaded(v + 3);
+            qk(g, 0, v + 3, true, t + 3 == n);
           }
         }
-        n0 += 2 * n;
-        pieces++;
       }
-      // nothing is in flight when the tensor memory is given back
-      tc_commit(&sh->fin);
-      bar_wait(sh, &sh->fin, 0, a.err, true);
+      n0 += 2 * n;
+      pieces++;
     }
+    // nothing is in flight when the tensor memory is given back
+    if (leader) tc_commit(&sh->fin);
     __syncwarp();
+    bar_wait(sh, &sh->fin, 0, a.err, true);
   } else {
     // ---- softmax: thread = row
     const int g = warp >> 2, row = tid & 127;
@@ -941,19 +988,27 @@ __global__ void __launch_bounds__(kTN, 1)
         bar_wait(sh, &sh->s_full[g], ns & 1, a.err);
         tc_fence_after();
         if (warp_on) {
-          float s[128];
-#pragma unroll
-          for (int c = 0; c < 4; c++) tc_ld32(s_at + 32 * c, s + 32 * c);
-          tc_wait_ld();
+          // the scores are read twice, once for the maximum and once for P: all
+          // 128 in registers would spill
           const int rel = lim - t * kTT;
-          if (__any_sync(0xffffffffu, rel < kTT)) {
+          const bool cut = __any_sync(0xffffffffu, rel < kTT);
+          float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 128; c++) s[c] = c < rel ? s[c] : -INFINITY;
+          for (int h = 0; h < 2; h++) {
+            uint32_t u[64];
+            float x[64];
+            tc_ld64(s_at + 64 * h, u);
+#pragma unroll
+            for (int c = 0; c < 64; c++) x[c] = __uint_as_float(u[c]);
+            if (cut)
+#pragma unroll
+              for (int c = 0; c < 64; c++) x[c] = 64 * h + c < rel ? x[c] : -INFINITY;
+            float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int c = 4; c < 64; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          top *= a.scale_log2;
           const bool raise = top > m + kSlack || m == -INFINITY;
           const float mn = raise ? fmaxf(m, top) : m;
           if (__any_sync(0xffffffffu, raise)) {
@@ -963,12 +1018,11 @@ __global__ void __launch_bounds__(kTN, 1)
               bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
               tc_fence_after();
               for (int c = 0; c < hd; c += 16) {
-                uint32_t o[16];
-                tc_ld16(o_at + c, o);
-                tc_wait_ld();
+                uint32_t u[16];
+                tc_ld16(o_at + c, u);
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tc_st16(o_at + c, o);
+                for (int e = 0; e < 16; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
+                tc_st16(o_at + c, u);
               }
             }
           }
@@ -977,18 +1031,28 @@ __global__ void __launch_bounds__(kTN, 1)
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int h = 0; h < 4; h++) {
-            uint32_t p[16], rest[16];
+            uint32_t u[32];
+            float x[32];
+            tc_ld32(s_at + 32 * h, u);
 #pragma unroll
-            for (int c = 0; c < 16; c++) {
-              const float x = ex2(fmaf(s[32 * h + 2 * c], a.scale_log2, -ms));
-              const float y = ex2(fmaf(s[32 * h + 2 * c + 1], a.scale_log2, -ms));
-              sum[2 * (c & 1)] += x;
-              sum[2 * (c & 1) + 1] += y;
-              p[c] = pack2<T>(x, y);
-              if (!both) rest[c] = pack2_rest<T>(x, y, p[c]);
+            for (int c = 0; c < 32; c++) x[c] = __uint_as_float(u[c]);
+            if (cut)
+#pragma unroll
+              for (int c = 0; c < 32; c++) x[c] = 32 * h + c < rel ? x[c] : -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 32; c++) {
+              x[c] = ex2(fmaf(x[c], a.scale_log2, -ms));
+              sum[c & 3] += x[c];
             }
-            tc_st16(s_at + 16 * h, p);
-            if (!both) tc_st16(s_at + 64 + 16 * h, rest);
+            uint32_t p[16];
+#pragma unroll
+            for (int c = 0; c < 16; c++) p[c] = pack2<T>(x[2 * c], x[2 * c + 1]);
+            tc_st16(s_at + 32 * h, p);
+            if (!both) {
+#pragma unroll
+              for (int c = 0; c < 16; c++) p[c] = pack2_rest<T>(x[2 * c], x[2 * c + 1], p[c]);
+              tc_st16(s_at + 32 * h + 16, p);
+            }
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tc_wait_st();
@@ -1009,16 +1073,15 @@ __global__ void __launch_bounds__(kTN, 1)
         const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
         if (warp_on)
           for (int c = 0; c < hd; c += 32) {
-            float o[32];
+            uint32_t o[32];
             tc_ld32(o_at + c, o);
-            tc_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
               if (mine && c + e < hd) {
                 uint32_t u[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                  const float x = o[e + 2 * k] * inv, y = o[e + 2 * k + 1] * inv;
+                  const float x = __uint_as_float(o[e + 2 * k]) * inv, y = __uint_as_float(o[e + 2 * k + 1]) * inv;
                   odd |= !isfinite(x) || !isfinite(y);
                   u[k] = pack2<T>(x, y);
                 }
@@ -1037,13 +1100,12 @@ __global__ void __launch_bounds__(kTN, 1)
       const int at = g * 128 + row;  // groups with the same rows leave two results
       if (warp_on && done)
         for (int c = 0; c < hd; c += 32) {
-          float o[32];
+          uint32_t o[32];
           tc_ld32(o_at + c, o);
-          tc_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             if (mine && c + e < hd)
-              *(float4 *)(dst + (size_t)at * kMaxHD + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              *(uint4 *)(dst + (size_t)at * kMaxHD + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       if (mine) {
         dst[kTR * kMaxHD + at] = m;

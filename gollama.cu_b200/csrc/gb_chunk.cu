@@ -70,17 +70,39 @@ struct Line {
     const int last = (int)min((long long)s.n * G, (long long)(u + 1) * RU) - 1;
     return max(1, (visible(s, G, last) + KT - 1) / KT);
   }
-  static GB_DEV long long seq_tiles(const ChunkArgs &a, int b) {
-    const Seq s = seq_of(a, b);
-    const int nu = units(s, a.G);
+  // Tiles of the sequences of this warp's lanes, over all KV heads (no rows: none). A sequence of many units is
+  // counted by the whole warp.
+  static GB_DEV long long seq_tiles(const ChunkArgs &a, const Seq &s) {
+    const int lane = threadIdx.x & 31, nu = units(s, a.G);
     long long t = 0;
-    for (int u = 0; u < nu; u++) t += tiles(s, a.G, u);
+    if (nu <= 4)
+      for (int u = 0; u < nu; u++) t += tiles(s, a.G, u);
+    for (unsigned many = __ballot_sync(0xffffffffu, nu > 4); many; many &= many - 1) {
+      const int from = __ffs(many) - 1;
+      Seq o;
+      o.q0 = 0, o.n = __shfl_sync(0xffffffffu, s.n, from), o.len0 = __shfl_sync(0xffffffffu, s.len0, from);
+      o.cap = __shfl_sync(0xffffffffu, s.cap, from);
+      const int no = units(o, a.G);
+      long long sum = 0;
+      for (int u = lane; u < no; u += 32) sum += tiles(o, a.G, u);
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+      if (lane == from) t = sum;
+    }
     return t * a.c.n_kv;
   }
 };
 
+// x * y / z, in 32 bits where x * y fits.
+GB_DEV long long mul_div(long long x, int y, long long z) {
+  const unsigned long long p = (unsigned long long)x * (unsigned)y;
+  if (p <= 0xFFFFFFFFull && z <= 0xFFFFFFFFll) return (uint32_t)p / (uint32_t)z;
+  return (long long)(p / (unsigned long long)z);
+}
+
 struct Plan {
-  long long total, ctas;    // the line's length, and the CTAs it is cut for
+  long long total;          // the line's length
+  int ctas;                 // the CTAs it is cut for
   long long x0, x1;         // this CTA's run of it
   long long rem;            // x0's place within its sequence
   int b;
@@ -103,13 +125,14 @@ GB_DEV long long block_scan(long long v, long long *warp_sums) {
 }
 
 // Every CTA finds its run by itself: each thread counts the tiles of a
-// sequence, and the sums of all of them are scanned. All NT threads call it.
+// sequence, and the sums of all of them are scanned (a kernel of its own for
+// it would cost a launch). All NT threads call it.
 template <int RU, int KT, int NT>
 GB_DEV void make_plan(const ChunkArgs &a, Plan *plan, long long *warp_sums) {
   const int tid = threadIdx.x, batch = a.c.batch;
   long long total = 0, first = 0, scan = 0;
   for (int b0 = 0; b0 < batch; b0 += NT) {
-    const long long v = b0 + tid < batch ? Line<RU, KT>::seq_tiles(a, b0 + tid) : 0;
+    const long long v = Line<RU, KT>::seq_tiles(a, b0 + tid < batch ? seq_of(a, b0 + tid) : Seq{0, 0, 0, 0});
     const long long s = block_scan<NT>(v, warp_sums);
     if (b0 == 0) first = v, scan = s;
     long long sum = 0;
@@ -118,13 +141,13 @@ GB_DEV void make_plan(const ChunkArgs &a, Plan *plan, long long *warp_sums) {
     __syncthreads();
   }
   // a line shorter than the grid goes to as many CTAs as it has tiles, so that no CTA amid a unit is without a piece
-  const long long ctas = min((long long)gridDim.x, total), me = min((long long)blockIdx.x, ctas);
-  const long long x0 = ctas ? total * me / ctas : 0, x1 = me < ctas ? total * (me + 1) / ctas : x0;
+  const int ctas = (int)min((long long)gridDim.x, total), me = min((int)blockIdx.x, ctas);
+  const long long x0 = ctas ? mul_div(total, me, ctas) : 0, x1 = me < ctas ? mul_div(total, me + 1, ctas) : x0;
   long long base = 0;
   for (int b0 = 0; b0 < batch; b0 += NT) {
     long long v = first, s = scan;
     if (batch > NT) {
-      v = b0 + tid < batch ? Line<RU, KT>::seq_tiles(a, b0 + tid) : 0;
+      v = Line<RU, KT>::seq_tiles(a, b0 + tid < batch ? seq_of(a, b0 + tid) : Seq{0, 0, 0, 0});
       s = block_scan<NT>(v, warp_sums);
     }
     if (v && base + s - v <= x0 && x0 < base + s) {
@@ -143,29 +166,48 @@ GB_DEV void make_plan(const ChunkArgs &a, Plan *plan, long long *warp_sums) {
 // A walk over the pieces of this CTA's run: a piece is a unit's tiles [t0, t1).
 template <int RU, int KT>
 struct Walk {
-  long long x, x1, total, ctas;
+  long long x, x1;
   int b, u, h, i;
   // the piece
   Seq s;
-  int r0, nr;           // the unit's packed rows [r0, r0 + nr) of the sequence
-  int head;             // its KV head
-  int t0, t1, nt;       // tiles of the piece, and of the unit
-  int c_first, c_last;  // CTAs that hold pieces of the unit
+  int r0, nr;      // the unit's packed rows [r0, r0 + nr) of the sequence
+  int head;        // its KV head
+  int t0, t1, nt;  // tiles of the piece, and of the unit
 
+  // All lanes of the warp call it: they look through the sequence's units 32 at a time.
   GB_DEV void start(const ChunkArgs &a, const Plan &p) {
-    x = p.x0, x1 = p.x1, total = p.total, ctas = p.ctas;
+    x = p.x0, x1 = p.x1;
     if (x >= x1) return;
     b = p.b;
     s = seq_of(a, b);
     long long rem = p.rem;
-    for (u = 0;; u++) {
-      nt = Line<RU, KT>::tiles(s, a.G, u);
-      const long long n = (long long)nt * a.c.n_kv;
-      if (rem < n) break;
-      rem -= n;
+    const int lane = threadIdx.x & 31, nu = Line<RU, KT>::units(s, a.G);
+    for (u = 0;; u += 32) {
+      const int mine = u + lane < nu ? Line<RU, KT>::tiles(s, a.G, u + lane) : 0;
+      long long sum = (long long)mine * a.c.n_kv;  // with the units before it
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, sum > rem);
+      if (past || u + 32 >= nu) {
+        const int at = past ? __ffs(past) - 1 : 0;
+        u += at;
+        nt = __shfl_sync(0xffffffffu, mine, at);
+        rem -= __shfl_sync(0xffffffffu, sum, at) - (long long)nt * a.c.n_kv;
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    h = (int)(rem / nt);
-    i = (int)(rem % nt);
+    h = (int)mul_div(rem, 1, nt);
+    i = (int)(rem - (long long)h * nt);
+  }
+  // The CTAs that hold pieces of the unit just returned (t0, t1).
+  GB_DEV void holders(const Plan &p, int *first, int *last) const {
+    const long long y0 = x - t1, y1 = y0 + nt;  // the unit's place in the line: x is where the piece ended
+    *first = (int)(((y0 + 1) * p.ctas - 1) / p.total);
+    *last = (int)((y1 * p.ctas - 1) / p.total);
   }
   GB_DEV bool next(const ChunkArgs &a) {
     if (x >= x1) return false;
@@ -183,9 +225,6 @@ struct Walk {
     head = h;
     t0 = i;
     t1 = (int)min((long long)nt, i + (x1 - x));
-    const long long y0 = x - i, y1 = y0 + nt;  // the unit's place in the line
-    c_first = (int)(((y0 + 1) * ctas - 1) / total);
-    c_last = (int)((y1 * ctas - 1) / total);
     x += t1 - t0;
     i = 0;
     h++;
@@ -206,8 +245,9 @@ GB_DEV long long pool_row(const ChunkArgs &a, const Seq &s, int b, int h, int p,
 // ---- partial rows ------------------------------------------------------------
 // A CTA leaves at most two pieces for others to join: the one its run begins
 // within (which = 0) and the one it begins and does not end (which = 1); a
-// third place (which = 2) is its own. Each has RU rows of kMaxHD floats, then
-// their maxima (of the scores in powers of two), then their sums.
+// third place (which = 2) is its own. Each holds kMaxHD floats of RU rows, four
+// dimensions of all rows after another (a warp's rows store 512 bytes at a
+// time), then the rows' maxima (of the scores in powers of two) and sums.
 constexpr int kMaxHD = 128, kPlaces = 3;
 template <int RU>
 GB_DEV float *part_slot(const ChunkArgs &a, int cta, int which) {
@@ -254,15 +294,17 @@ GB_DEV void ld4(const void *base, long long i, float *o) {
   }
 }
 
-// One row by itself, by one warp: lane = position for the scores, lane = four
-// dimensions for the sum over V. Taken for rows that came out with an infinity
-// or NaN: a tile holds positions that some of its rows do not see, and their
-// weight of zero does not stop a NaN or an infinity in V. Here the row meets
-// nothing but its own positions, so what it shows is its own.
+// One row by itself, by one warp: lane = position for the scores, then lane =
+// four dimensions for the sum over V (all of the row, c4 < 0), or lane =
+// position for the dimensions 4 c4.. alone. Taken for what came out as an
+// infinity or NaN: a tile holds positions that some of its rows do not see, and
+// their weight of zero does not stop a NaN or an infinity in V. Here the row
+// meets nothing but its own positions, so what it shows is its own.
 template <int T>
-__device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, int head, int pr) {
+__device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, int head, int pr, int c4) {
   const int lane = threadIdx.x & 31, hd = a.c.head_dim, lim = visible(s, a.G, pr);
   const long long row = s.q0 + pr / a.G, hq = (long long)(head * a.G + pr % a.G) * hd;
+  const int my4 = c4 < 0 ? lane : c4;
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = 0; p0 < lim; p0 += 32) {
     const int p = p0 + lane;
@@ -280,65 +322,74 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
     l = fmaf(l, f, gb_warp_sum(e));
     m = mn;
     for (int k = 0; k < 4; k++) o[k] *= f;
-    const int n = min(32, lim - p0);
+    const int n = c4 < 0 ? min(32, lim - p0) : 1;
     for (int j = 0; j < n; j++) {
-      const float pj = __shfl_sync(0xffffffffu, e, j);
-      const long long vj = __shfl_sync(0xffffffffu, at, j);
-      if (4 * lane < hd && vj >= 0) {
+      const int from = c4 < 0 ? j : lane;
+      const float pj = __shfl_sync(0xffffffffu, e, from);
+      const long long vj = __shfl_sync(0xffffffffu, at, from);
+      if (4 * my4 < hd && vj >= 0) {
         float v[4];
-        ld4<T>(a.c.v_pool, vj + 4 * lane, v);
+        ld4<T>(a.c.v_pool, vj + 4 * my4, v);
         for (int k = 0; k < 4; k++) o[k] = fmaf(pj, v[k], o[k]);
       }
     }
   }
+  if (c4 >= 0)
+    for (int k = 0; k < 4; k++) o[k] = gb_warp_sum(o[k]);
   const float inv = lim > 0 ? 1.f / l : 0.f;
-  if (4 * lane < hd) put4<T>(a.out, row * a.ldo + hq + 4 * lane, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (4 * my4 < hd && (c4 < 0 || lane == 0))
+    put4<T>(a.out, row * a.ldo + hq + 4 * my4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
-// Joins the pieces of a unit, CTA by CTA: one warp to a row, four dimensions
-// to a lane. With HALVES a place holds two pieces of the same rows, RU / 2
-// rows apart. `own`: the unit is this CTA's alone, in its own place.
+// Joins the pieces of a unit, CTA by CTA: a thread takes four dimensions of a
+// row, neighbours the next row's. With HALVES a place holds two pieces of the
+// same rows, RU / 2 rows apart. `own`: the unit is this CTA's alone, in its own
+// place. NT threads, the first warps of the block.
 struct Unit {
   Seq s;
   int b, head, r0, nr, c_first, c_last;
+  bool own;
 };
-template <int T, int RU, bool HALVES>
-__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int warp, int warps, bool own) {
-  const int lane = threadIdx.x & 31, hd = a.c.head_dim;
-  const int c0 = own ? (int)blockIdx.x : w.c_first, c1 = own ? (int)blockIdx.x : w.c_last;
-  const int parts = HALVES ? 2 : 1, n = (c1 - c0 + 1) * parts;
-  for (int r = warp; r < w.nr; r += warps) {
-    auto place = [&](int i) {
-      const int c = c0 + i / parts;
-      return part_slot<RU>(a, c, own ? 2 : c == c0);
-    };
-    auto row = [&](int i) { return r + i % parts * (RU / 2); };
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(place(i) + RU * kMaxHD + row(i)));
-    m = gb_warp_max(m);
-    if (m == -INFINITY) m = 0.f;
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < n; i++) {
-      const float *p = place(i);
-      const float mi = __ldcg(p + RU * kMaxHD + row(i)), li = __ldcg(p + RU * (kMaxHD + 1) + row(i));
-      const float4 v = __ldcg((const float4 *)(p + (size_t)row(i) * kMaxHD) + lane);
-      if (mi == -INFINITY && li == 0.f) continue;  // nothing seen there; its outputs may not have been written
-      const float f = ex2(mi - m);
-      l = fmaf(f, li, l);
-      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int pr = w.r0 + r;
+template <int T, int RU, bool HALVES, int NT>
+__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid) {
+  const int hd = a.c.head_dim, c0 = w.own ? (int)blockIdx.x : w.c_first;
+  const int parts = HALVES ? 2 : 1, n = w.own ? parts : (w.c_last - c0 + 1) * parts, items = w.nr * (hd / 4);
+  auto place = [&](int i) {
+    const int c = c0 + i / parts;
+    return part_slot<RU>(a, c, w.own ? 2 : c == c0);
+  };
+  for (int i0 = 0; i0 < items; i0 += NT) {
+    const int item = i0 + tid, r = item % w.nr, c4 = item / w.nr, pr = w.r0 + r;
     bool odd = false;
-    if (4 * lane < hd) {
-      const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd + 4 * lane;
+    if (item < items) {
+      float m = -INFINITY;
+#pragma unroll 4
+      for (int i = 0; i < n; i++) m = fmaxf(m, __ldcg(place(i) + RU * kMaxHD + r + i % parts * (RU / 2)));
+      if (m == -INFINITY) m = 0.f;
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int i = 0; i < n; i++) {
+        const int at = r + i % parts * (RU / 2);
+        const float *p = place(i);
+        const float mi = __ldcg(p + RU * kMaxHD + at), li = __ldcg(p + RU * (kMaxHD + 1) + at);
+        const float4 v = __ldcg((const float4 *)p + (size_t)c4 * RU + at);
+        if (mi == -INFINITY && li == 0.f) continue;  // nothing seen there; its outputs may not have been written
+        const float f = ex2(mi - m);
+        l = fmaf(f, li, l);
+        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+      }
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd + 4 * c4;
       o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
       put4<T>(a.out, at, o.x, o.y, o.z, o.w);
       odd = !isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w);
     }
-    if (__any_sync(0xffffffffu, odd)) redo_row<T>(a, w.s, w.b, w.head, pr);
+    __syncwarp();
+    for (unsigned any = __ballot_sync(0xffffffffu, odd); any; any &= any - 1) {
+      const int from = __ffs(any) - 1;
+      redo_row<T>(a, w.s, w.b, w.head, __shfl_sync(0xffffffffu, pr, from), __shfl_sync(0xffffffffu, c4, from));
+    }
   }
 }
 
@@ -481,7 +532,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
 #pragma unroll
         for (int half = 0; half < 2; half++)
           if (any >> (16 * half) & 0xFFFFu)
-            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r);
+            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r, -1);
       }
       continue;
     }
@@ -491,21 +542,23 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
       if (4 * ty + r >= w.nr) continue;
 #pragma unroll
       for (int j = 0; j < HD / 64; j++)
-        *(float4 *)(dst + (size_t)(4 * ty + r) * kMaxHD + 64 * j + 4 * tx) =
+        *(float4 *)(dst + ((size_t)(16 * j + tx) * kCR + 4 * ty + r) * 4) =
             make_float4(o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]);
       if (tx == 0) {
         dst[kCR * kMaxHD + 4 * ty + r] = m[r];
         dst[kCR * (kMaxHD + 1) + 4 * ty + r] = l[r];
       }
     }
+    int c_first, c_last;
+    w.holders(plan, &c_first, &c_last);
     __threadfence();
     __syncthreads();
-    if (tid == 0) arrived = atomicAdd(a.counter + w.c_first, 1u);
+    if (tid == 0) arrived = atomicAdd(a.counter + c_first, 1u);
     __syncthreads();
-    if (arrived != (unsigned)(w.c_last - w.c_first)) continue;
+    if (arrived != (unsigned)(c_last - c_first)) continue;
     __threadfence();
-    join_pieces<GB_F32, kCR, false>(a, {w.s, w.b, w.head, w.r0, w.nr, w.c_first, w.c_last}, tid >> 5, kCN / 32, false);
-    if (tid == 0) a.counter[w.c_first] = 0u;  // ready for the next launch
+    join_pieces<GB_F32, kCR, false, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last, false}, tid);
+    if (tid == 0) a.counter[c_first] = 0u;  // ready for the next launch
   }
 }
 
@@ -740,6 +793,97 @@ GB_DEV uint32_t pack2_rest(float x, float y, uint32_t p) {
   } else {
     return pack2<T>(x - __uint_as_float(p << 16), y - __uint_as_float(p & 0xFFFF0000u));
   }
+}
+
+// Two float32 in one register pair.
+GB_DEV uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+GB_DEV void unpair(uint64_t r, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+GB_DEV uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+GB_DEV uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+GB_DEV float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+// 2^x of a pair without the exponential unit: x = n + f with n whole and f in
+// [-1/2, 1/2] (the sum with 1.5 2^23 leaves n in the low bits), 2^f by the
+// polynomial of degree 4 of least relative error there (2.7e-6, a ninetieth of
+// binary16's half step), n added to the exponent. Below -126 it stays there; of
+// a NaN it makes the largest number, an infinity in P: the row is done again.
+GB_DEV uint64_t ex2_poly(uint64_t x) {
+  float x0, x1, r0, r1, p0, p1;
+  unpair(x, x0, x1);
+  const uint64_t t = pair(max_nan(x0, -126.f), max_nan(x1, -126.f));
+  const uint64_t r = add2(t, pair(12582912.f, 12582912.f)), n = add2(r, pair(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pair(-1.f, -1.f), t);
+  uint64_t p = pair(0x1.3997b4p-7f, 0x1.3997b4p-7f);
+  p = fma2(p, f, pair(0x1.ca143cp-5f, 0x1.ca143cp-5f));
+  p = fma2(p, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = fma2(p, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = fma2(p, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  unpair(r, r0, r1);
+  unpair(p, p0, p1);
+  return pair(__uint_as_float((__float_as_uint(r0) << 23) + __float_as_uint(p0)),
+              __uint_as_float((__float_as_uint(r1) << 23) + __float_as_uint(p1)));
+}
+
+// P of this warp's rows from the scores at s_at, in their place: powers of two
+// of s * scale + shift, rounded to T (and the remainders, unless `both`); the
+// sum of a row's. CUT: columns from `rel` on are not seen. The exponential unit
+// does four a clock and scheduler, 1024 clocks for a warp's 128 columns: as long
+// as the tensor cores take for both products. So of each eight columns two go
+// through ex2_poly on the multiply-add units.
+template <int T, bool CUT>
+GB_DEV float weights(uint32_t s_at, bool both, int rel, float scale, float shift) {
+  const uint64_t k2 = pair(scale, scale), c2 = pair(shift, shift);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    uint32_t u[64];
+    tc_ld64(s_at + 64 * h, u);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      uint32_t p[16], rest[16];
+#pragma unroll
+      for (int c = 0; c < 16; c++) {
+        const int at = 32 * k + 2 * c;
+        float x = __uint_as_float(u[at]), y = __uint_as_float(u[at + 1]);
+        if (CUT) {
+          x = 64 * h + at < rel ? x : -INFINITY;
+          y = 64 * h + at + 1 < rel ? y : -INFINITY;
+        }
+        uint64_t e = fma2(pair(x, y), k2, c2);
+        if (!CUT && c % 4 == 3) {
+          e = ex2_poly(e);
+          unpair(e, x, y);
+        } else {
+          unpair(e, x, y);
+          x = ex2(x), y = ex2(y);
+          e = pair(x, y);
+        }
+        sum[c & 1] = add2(sum[c & 1], e);
+        p[c] = pack2<T>(x, y);
+        if (!both) rest[c] = pack2_rest<T>(x, y, p[c]);
+      }
+      tc_st16(s_at + 64 * h + 32 * k, p);
+      if (!both) tc_st16(s_at + 64 * h + 32 * k + 16, rest);
+    }
+  }
+  float x, y;
+  unpair(add2(sum[0], sum[1]), x, y);
+  return x + y;
 }
 
 template <int T, int HD, bool TMA>
@@ -1028,33 +1172,8 @@ __global__ void __launch_bounds__(kTN, 1)
           }
           m = mn;
           const float ms = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int h = 0; h < 4; h++) {
-            uint32_t u[32];
-            float x[32];
-            tc_ld32(s_at + 32 * h, u);
-#pragma unroll
-            for (int c = 0; c < 32; c++) x[c] = __uint_as_float(u[c]);
-            if (cut)
-#pragma unroll
-              for (int c = 0; c < 32; c++) x[c] = 32 * h + c < rel ? x[c] : -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 32; c++) {
-              x[c] = ex2(fmaf(x[c], a.scale_log2, -ms));
-              sum[c & 3] += x[c];
-            }
-            uint32_t p[16];
-#pragma unroll
-            for (int c = 0; c < 16; c++) p[c] = pack2<T>(x[2 * c], x[2 * c + 1]);
-            tc_st16(s_at + 32 * h, p);
-            if (!both) {
-#pragma unroll
-              for (int c = 0; c < 16; c++) p[c] = pack2_rest<T>(x[2 * c], x[2 * c + 1], p[c]);
-              tc_st16(s_at + 32 * h + 16, p);
-            }
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if (cut) l += weights<T, true>(s_at, both, rel, a.scale_log2, -ms);
+          else l += weights<T, false>(s_at, both, rel, a.scale_log2, -ms);
           tc_wait_st();
         }
         tc_fence_before();
@@ -1092,7 +1211,7 @@ __global__ void __launch_bounds__(kTN, 1)
         __syncwarp();
         if (lane == 0) gb_mbar_arrive(&sh->o_free[g]);
         for (unsigned any = __ballot_sync(0xffffffffu, odd); any; any &= any - 1)
-          redo_row<T>(a, w.s, w.b, w.head, pr - lane + __ffs(any) - 1);
+          redo_row<T>(a, w.s, w.b, w.head, pr - lane + __ffs(any) - 1, -1);
         continue;
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the CTA's own place has been read out
@@ -1105,7 +1224,7 @@ __global__ void __launch_bounds__(kTN, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             if (mine && c + e < hd)
-              *(uint4 *)(dst + (size_t)at * kMaxHD + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              *(uint4 *)(dst + ((size_t)((c + e) >> 2) * kTR + at) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       if (mine) {
         dst[kTR * kMaxHD + at] = m;
@@ -1116,16 +1235,17 @@ __global__ void __launch_bounds__(kTN, 1)
       if (lane == 0) gb_mbar_arrive(&sh->o_free[g]);
       __threadfence();
       asm volatile("bar.sync 1, 256;" ::: "memory");
+      Unit unit = {w.s, w.b, w.head, w.r0, w.nr, 0, 0, whole};
       if (!whole) {
-        if (tid == 0) sh->arrived = atomicAdd(a.counter + w.c_first, 1u);
+        w.holders(sh->plan, &unit.c_first, &unit.c_last);
+        if (tid == 0) sh->arrived = atomicAdd(a.counter + unit.c_first, 1u);
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (sh->arrived != (unsigned)(w.c_last - w.c_first)) continue;
+        if (sh->arrived != (unsigned)(unit.c_last - unit.c_first)) continue;
         __threadfence();
       }
-      const Unit unit = {w.s, w.b, w.head, w.r0, w.nr, w.c_first, w.c_last};
-      if (both) join_pieces<T, kTR, false>(a, unit, warp, kSoftWarps, whole);
-      else join_pieces<T, kTR, true>(a, unit, warp, kSoftWarps, whole);
-      if (!whole && tid == 0) a.counter[w.c_first] = 0u;  // ready for the next launch
+      if (both) join_pieces<T, kTR, false, kSoftWarps * 32>(a, unit, tid);
+      else join_pieces<T, kTR, true, kSoftWarps * 32>(a, unit, tid);
+      if (!whole && tid == 0) a.counter[unit.c_first] = 0u;  // ready for the next launch
     }
   }
   tc_fence_before();

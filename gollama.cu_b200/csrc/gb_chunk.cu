@@ -341,8 +341,8 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
     put4<T>(a.out, row * a.ldo + hq + 4 * my4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
-// Joins the pieces of a unit, CTA by CTA: a thread takes four dimensions of a
-// row, neighbours the next row's. With HALVES a place holds two pieces of the
+// Joins the pieces of a unit, CTA by CTA: neighbour threads take neighbour rows,
+// each all of its row's dimensions or, with few rows, every so many. With HALVES a place holds two pieces of the
 // same rows, RU / 2 rows apart. `own`: the unit is this CTA's alone, in its own
 // place. NT threads, the first warps of the block.
 struct Unit {
@@ -352,43 +352,68 @@ struct Unit {
 };
 template <int T, int RU, bool HALVES, int NT>
 __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid) {
-  const int hd = a.c.head_dim, c0 = w.own ? (int)blockIdx.x : w.c_first;
-  const int parts = HALVES ? 2 : 1, n = w.own ? parts : (w.c_last - c0 + 1) * parts, items = w.nr * (hd / 4);
+  const int hd = a.c.head_dim, c0 = w.own ? (int)blockIdx.x : w.c_first, n4 = hd / 4;
+  const int parts = HALVES ? 2 : 1, n = w.own ? parts : (w.c_last - c0 + 1) * parts;
   auto place = [&](int i) {
     const int c = c0 + i / parts;
     return part_slot<RU>(a, c, w.own ? 2 : c == c0);
   };
-  for (int i0 = 0; i0 < items; i0 += NT) {
-    const int item = i0 + tid, r = item % w.nr, c4 = item / w.nr, pr = w.r0 + r;
-    bool odd = false;
-    if (item < items) {
-      float m = -INFINITY;
-#pragma unroll 4
+  // threads to a row: a power of two, so that few rows spread over all threads
+  int split = 1;
+  while (split < 32 && 2 * split * w.nr <= NT) split *= 2;
+  for (int i0 = 0; i0 < w.nr * split; i0 += NT) {
+    const int item = i0 + tid, r = item % w.nr, sub = item / w.nr, pr = w.r0 + r;
+    const bool on = sub < split;
+    unsigned odd = 0;
+    if (on) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 8
       for (int i = 0; i < n; i++) m = fmaxf(m, __ldcg(place(i) + RU * kMaxHD + r + i % parts * (RU / 2)));
       if (m == -INFINITY) m = 0.f;
-      float l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
       for (int i = 0; i < n; i++) {
-        const int at = r + i % parts * (RU / 2);
-        const float *p = place(i);
-        const float mi = __ldcg(p + RU * kMaxHD + at), li = __ldcg(p + RU * (kMaxHD + 1) + at);
-        const float4 v = __ldcg((const float4 *)p + (size_t)c4 * RU + at);
-        if (mi == -INFINITY && li == 0.f) continue;  // nothing seen there; its outputs may not have been written
-        const float f = ex2(mi - m);
-        l = fmaf(f, li, l);
-        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+        const float *p = place(i) + RU * kMaxHD + r + i % parts * (RU / 2);
+        l = fmaf(ex2(__ldcg(p) - m), __ldcg(p + RU), l);
       }
       const float inv = l != 0.f ? 1.f / l : 0.f;
-      const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd + 4 * c4;
-      o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-      put4<T>(a.out, at, o.x, o.y, o.z, o.w);
-      odd = !isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w);
+      const long long row = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
+      // four runs of four dimensions at a time: their loads are all on their way together
+      for (int q0 = sub; q0 < n4; q0 += 4 * split) {
+        float4 o[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+          const int at = r + i % parts * (RU / 2);
+          const float *p = place(i);
+          const float mi = __ldcg(p + RU * kMaxHD + at), li = __ldcg(p + RU * (kMaxHD + 1) + at);
+          float4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (q0 + k * split < n4) v[k] = __ldcg((const float4 *)p + (size_t)(q0 + k * split) * RU + at);
+          if (mi == -INFINITY && li == 0.f) continue;  // nothing seen there; its outputs may not have been written
+          const float f = ex2(mi - m) * inv;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            o[k].x = fmaf(f, v[k].x, o[k].x), o[k].y = fmaf(f, v[k].y, o[k].y);
+            o[k].z = fmaf(f, v[k].z, o[k].z), o[k].w = fmaf(f, v[k].w, o[k].w);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int c4 = q0 + k * split;
+          if (c4 >= n4) continue;
+          put4<T>(a.out, row + 4 * c4, o[k].x, o[k].y, o[k].z, o[k].w);
+          if (!isfinite(o[k].x) || !isfinite(o[k].y) || !isfinite(o[k].z) || !isfinite(o[k].w)) odd |= 1u << c4;
+        }
+      }
     }
     __syncwarp();
-    for (unsigned any = __ballot_sync(0xffffffffu, odd); any; any &= any - 1) {
+    for (unsigned any = __ballot_sync(0xffffffffu, odd != 0); any; any &= any - 1) {
       const int from = __ffs(any) - 1;
-      redo_row<T>(a, w.s, w.b, w.head, __shfl_sync(0xffffffffu, pr, from), __shfl_sync(0xffffffffu, c4, from));
+      const int rr = __shfl_sync(0xffffffffu, pr, from);
+      for (unsigned which = __shfl_sync(0xffffffffu, odd, from); which; which &= which - 1)
+        redo_row<T>(a, w.s, w.b, w.head, rr, __ffs(which) - 1);
     }
   }
 }
@@ -844,42 +869,39 @@ GB_DEV uint64_t ex2_poly(uint64_t x) {
 // sum of a row's. CUT: columns from `rel` on are not seen. The exponential unit
 // does four a clock and scheduler, 1024 clocks for a warp's 128 columns: as long
 // as the tensor cores take for both products. So of each eight columns two go
-// through ex2_poly on the multiply-add units.
+// through ex2_poly on the multiply-add units. The loops stay rolled: straight
+// code for 128 columns outgrows the schedulers' instruction caches, and fetching
+// it took as long as running it (stalls on no instruction as many as issues).
 template <int T, bool CUT>
 GB_DEV float weights(uint32_t s_at, bool both, int rel, float scale, float shift) {
   const uint64_t k2 = pair(scale, scale), c2 = pair(shift, shift);
   uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+  for (int h = 0; h < 4; h++) {
+    uint32_t u[32], p[16];
+    tc_ld32(s_at + 32 * h, u);
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    uint32_t u[64];
-    tc_ld64(s_at + 64 * h, u);
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      uint32_t p[16], rest[16];
-#pragma unroll
-      for (int c = 0; c < 16; c++) {
-        const int at = 32 * k + 2 * c;
-        float x = __uint_as_float(u[at]), y = __uint_as_float(u[at + 1]);
-        if (CUT) {
-          x = 64 * h + at < rel ? x : -INFINITY;
-          y = 64 * h + at + 1 < rel ? y : -INFINITY;
-        }
-        uint64_t e = fma2(pair(x, y), k2, c2);
-        if (!CUT && c % 4 == 3) {
-          e = ex2_poly(e);
-          unpair(e, x, y);
-        } else {
-          unpair(e, x, y);
-          x = ex2(x), y = ex2(y);
-          e = pair(x, y);
-        }
-        sum[c & 1] = add2(sum[c & 1], e);
-        p[c] = pack2<T>(x, y);
-        if (!both) rest[c] = pack2_rest<T>(x, y, p[c]);
+    for (int c = 0; c < 16; c++) {
+      float x = __uint_as_float(u[2 * c]), y = __uint_as_float(u[2 * c + 1]);
+      if (CUT) {
+        x = 32 * h + 2 * c < rel ? x : -INFINITY;
+        y = 32 * h + 2 * c + 1 < rel ? y : -INFINITY;
       }
-      tc_st16(s_at + 64 * h + 32 * k, p);
-      if (!both) tc_st16(s_at + 64 * h + 32 * k + 16, rest);
+      uint64_t e = fma2(pair(x, y), k2, c2);
+      if (!CUT && c % 4 == 3) {
+        e = ex2_poly(e);
+        unpair(e, x, y);
+      } else {
+        unpair(e, x, y);
+        x = ex2(x), y = ex2(y);
+        e = pair(x, y);
+      }
+      sum[c & 1] = add2(sum[c & 1], e);
+      p[c] = pack2<T>(x, y);
+      if (!both) u[c] = pack2_rest<T>(x, y, p[c]);
     }
+    tc_st16(s_at + 32 * h, p);
+    if (!both) tc_st16(s_at + 32 * h + 16, u);
   }
   float x, y;
   unpair(add2(sum[0], sum[1]), x, y);
@@ -1086,12 +1108,10 @@ __global__ void __launch_bounds__(kTN, 1)
         loaded(v);
         if (both) {
           if (t == 0) bar_wait(sh, &sh->o_free[0], free_parity, a.err);
+          if (t + 1 < n) loaded(v + 1);
           p_ready(0);
           pv(0, v, t == 0, true, false);
-          if (t + 1 < n) {
-            loaded(v + 1);
-            qk(0, 0, v + 1, false, false);
-          }
+          if (t + 1 < n) qk(0, 0, v + 1, false, false);
           if (t == 0) bar_wait(sh, &sh->o_free[1], free_parity, a.err);
           p_ready(1);
           pv(1, v, t == 0, true, true);
@@ -1137,7 +1157,7 @@ __global__ void __launch_bounds__(kTN, 1)
           const int rel = lim - t * kTT;
           const bool cut = __any_sync(0xffffffffu, rel < kTT);
           float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
           for (int h = 0; h < 2; h++) {
             uint32_t u[64];
             float x[64];

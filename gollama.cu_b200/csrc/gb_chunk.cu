@@ -244,11 +244,11 @@ GB_DEV long long pool_row(const ChunkArgs &a, const Seq &s, int b, int h, int p,
 
 // ---- partial rows ------------------------------------------------------------
 // A CTA leaves at most two pieces for others to join: the one its run begins
-// within (which = 0) and the one it begins and does not end (which = 1); a
-// third place (which = 2) is its own. Each holds kMaxHD floats of RU rows, four
+// within (which = 0) and the one it begins and does not end (which = 1). Each
+// place holds kMaxHD floats of RU rows, four
 // dimensions of all rows after another (a warp's rows store 512 bytes at a
 // time), then the rows' maxima (of the scores in powers of two) and sums.
-constexpr int kMaxHD = 128, kPlaces = 3;
+constexpr int kMaxHD = 128, kPlaces = 2;
 template <int RU>
 GB_DEV float *part_slot(const ChunkArgs &a, int cta, int which) {
   return a.part + (size_t)(cta * kPlaces + which) * RU * (kMaxHD + 2);
@@ -273,38 +273,38 @@ GB_DEV void put4(void *out, long long i, float x, float y, float z, float w) {
   }
 }
 
+// Four elements of type T from their 16 or 8 bytes.
+template <int T>
+GB_DEV void four(const uint4 &u, float *o) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if constexpr (T == GB_F32) o[e] = __uint_as_float(w[e]);
+    else if constexpr (T == GB_F16) o[e] = gb_half_to_float((uint16_t)(w[e / 2] >> 16 * (e & 1)));
+    else o[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+  }
+}
 template <int T>
 GB_DEV void ld4(const void *base, long long i, float *o) {
   if constexpr (T == GB_F32) {
-    const float4 x = __ldg((const float4 *)((const float *)base + i));
-    o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
+    four<T>(__ldg((const uint4 *)((const float *)base + i)), o);
   } else {
     const uint2 u = __ldg((const uint2 *)((const uint16_t *)base + i));
-    const uint32_t w[2] = {u.x, u.y};
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      if constexpr (T == GB_F16) {
-        o[2 * e] = gb_half_to_float((uint16_t)w[e]);
-        o[2 * e + 1] = gb_half_to_float((uint16_t)(w[e] >> 16));
-      } else {
-        o[2 * e] = __uint_as_float(w[e] << 16);
-        o[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-      }
-    }
+    four<T>(make_uint4(u.x, u.y, 0, 0), o);
   }
 }
 
 // One row by itself, by one warp: lane = position for the scores, then lane =
-// four dimensions for the sum over V (all of the row, c4 < 0), or lane =
-// position for the dimensions 4 c4.. alone. Taken for what came out as an
+// four dimensions for the sum over V, of which it writes those of the mask's
+// bits (lane = position still, where that is one). Taken for what came out as an
 // infinity or NaN: a tile holds positions that some of its rows do not see, and
 // their weight of zero does not stop a NaN or an infinity in V. Here the row
 // meets nothing but its own positions, so what it shows is its own.
 template <int T>
-__device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, int head, int pr, int c4) {
+__device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, int head, int pr, unsigned mask) {
   const int lane = threadIdx.x & 31, hd = a.c.head_dim, lim = visible(s, a.G, pr);
   const long long row = s.q0 + pr / a.G, hq = (long long)(head * a.G + pr % a.G) * hd;
-  const int my4 = c4 < 0 ? lane : c4;
+  const int c4 = __popc(mask) == 1 ? __ffs(mask) - 1 : -1, my4 = c4 < 0 ? lane : c4;
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = 0; p0 < lim; p0 += 32) {
     const int p = p0 + lane;
@@ -337,85 +337,95 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
   if (c4 >= 0)
     for (int k = 0; k < 4; k++) o[k] = gb_warp_sum(o[k]);
   const float inv = lim > 0 ? 1.f / l : 0.f;
-  if (4 * my4 < hd && (c4 < 0 || lane == 0))
+  if (4 * my4 < hd && (c4 < 0 ? mask >> lane & 1 : lane == 0))
     put4<T>(a.out, row * a.ldo + hq + 4 * my4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
-// Joins the pieces of a unit, CTA by CTA: neighbour threads take neighbour rows,
-// each all of its row's dimensions or, with few rows, every so many. With HALVES a place holds two pieces of the
-// same rows, RU / 2 rows apart. `own`: the unit is this CTA's alone, in its own
-// place. NT threads, the first warps of the block.
 struct Unit {
   Seq s;
   int b, head, r0, nr, c_first, c_last;
-  bool own;
 };
-template <int T, int RU, bool HALVES, int NT>
-__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid) {
-  const int hd = a.c.head_dim, c0 = w.own ? (int)blockIdx.x : w.c_first, n4 = hd / 4;
-  const int parts = HALVES ? 2 : 1, n = w.own ? parts : (w.c_last - c0 + 1) * parts;
-  auto place = [&](int i) {
-    const int c = c0 + i / parts;
-    return part_slot<RU>(a, c, w.own ? 2 : c == c0);
-  };
-  // threads to a row: a power of two, so that few rows spread over all threads
-  int split = 1;
+// The joined rows of a unit, the block's first NT threads calling: neighbour
+// threads take neighbour rows, each all of its row's dimensions or, with few
+// rows, every so many. KC runs of four dimensions by PB pieces are loaded
+// together.
+template <int T, int RU, int NT, int KC, int PB>
+GB_DEV void join_rows(const ChunkArgs &a, const Unit &w, int tid) {
+  const int hd = a.c.head_dim, n4 = hd / 4, n = w.c_last - w.c_first + 1;
+  int split = 1;  // threads to a row
   while (split < 32 && 2 * split * w.nr <= NT) split *= 2;
   for (int i0 = 0; i0 < w.nr * split; i0 += NT) {
     const int item = i0 + tid, r = item % w.nr, sub = item / w.nr, pr = w.r0 + r;
-    const bool on = sub < split;
     unsigned odd = 0;
-    if (on) {
-      float m = -INFINITY, l = 0.f;
-#pragma unroll 8
-      for (int i = 0; i < n; i++) m = fmaxf(m, __ldcg(place(i) + RU * kMaxHD + r + i % parts * (RU / 2)));
-      if (m == -INFINITY) m = 0.f;
-#pragma unroll 8
-      for (int i = 0; i < n; i++) {
-        const float *p = place(i) + RU * kMaxHD + r + i % parts * (RU / 2);
-        l = fmaf(ex2(__ldcg(p) - m), __ldcg(p + RU), l);
-      }
-      const float inv = l != 0.f ? 1.f / l : 0.f;
+    if (sub < split) {
       const long long row = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
-      // four runs of four dimensions at a time: their loads are all on their way together
-      for (int q0 = sub; q0 < n4; q0 += 4 * split) {
-        float4 o[4];
+      for (int q0 = sub; q0 < n4; q0 += KC * split) {
+        float m = -INFINITY, l = 0.f;
+        float4 o[KC];
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = 0; i < n; i++) {
-          const int at = r + i % parts * (RU / 2);
-          const float *p = place(i);
-          const float mi = __ldcg(p + RU * kMaxHD + at), li = __ldcg(p + RU * (kMaxHD + 1) + at);
-          float4 v[4];
+        for (int k = 0; k < KC; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < n; p0 += PB) {
+          float mi[PB], li[PB];
+          float4 v[PB][KC];
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            if (q0 + k * split < n4) v[k] = __ldcg((const float4 *)p + (size_t)(q0 + k * split) * RU + at);
-          if (mi == -INFINITY && li == 0.f) continue;  // nothing seen there; its outputs may not have been written
-          const float f = ex2(mi - m) * inv;
+          for (int i = 0; i < PB; i++) {
+            mi[i] = -INFINITY, li[i] = 0.f;
+            if (p0 + i < n) {
+              const int c = w.c_first + p0 + i;
+              const uint32_t p = (uint32_t)(c * kPlaces + (c == w.c_first)) * (RU * (kMaxHD + 2));  // below 2^24
+              mi[i] = __ldcg(a.part + (p + RU * kMaxHD + r)), li[i] = __ldcg(a.part + (p + RU * (kMaxHD + 1) + r));
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            o[k].x = fmaf(f, v[k].x, o[k].x), o[k].y = fmaf(f, v[k].y, o[k].y);
-            o[k].z = fmaf(f, v[k].z, o[k].z), o[k].w = fmaf(f, v[k].w, o[k].w);
+              for (int k = 0; k < KC; k++)
+                if (q0 + k * split < n4)
+                  v[i][k] = __ldcg((const float4 *)(a.part + (p + ((q0 + k * split) * RU + r) * 4)));
+            }
+          }
+          float mn = m;
+#pragma unroll
+          for (int i = 0; i < PB; i++) mn = fmaxf(mn, mi[i]);
+          const float ms = mn == -INFINITY ? 0.f : mn, g = ex2(m - ms);
+          m = mn;
+          l *= g;
+#pragma unroll
+          for (int k = 0; k < KC; k++) o[k].x *= g, o[k].y *= g, o[k].z *= g, o[k].w *= g;
+#pragma unroll
+          for (int i = 0; i < PB; i++) {
+            if (mi[i] == -INFINITY && li[i] == 0.f) continue;  // nothing seen there: its outputs may not be written
+            const float f = ex2(mi[i] - ms);
+            l = fmaf(f, li[i], l);
+#pragma unroll
+            for (int k = 0; k < KC; k++) {
+              o[k].x = fmaf(f, v[i][k].x, o[k].x), o[k].y = fmaf(f, v[i][k].y, o[k].y);
+              o[k].z = fmaf(f, v[i][k].z, o[k].z), o[k].w = fmaf(f, v[i][k].w, o[k].w);
+            }
           }
         }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < KC; k++) {
           const int c4 = q0 + k * split;
           if (c4 >= n4) continue;
-          put4<T>(a.out, row + 4 * c4, o[k].x, o[k].y, o[k].z, o[k].w);
-          if (!isfinite(o[k].x) || !isfinite(o[k].y) || !isfinite(o[k].z) || !isfinite(o[k].w)) odd |= 1u << c4;
+          const float x = o[k].x * inv, y = o[k].y * inv, z = o[k].z * inv, u = o[k].w * inv;
+          put4<T>(a.out, row + 4 * c4, x, y, z, u);
+          if (!isfinite(x) || !isfinite(y) || !isfinite(z) || !isfinite(u)) odd |= 1u << c4;
         }
       }
     }
     __syncwarp();
     for (unsigned any = __ballot_sync(0xffffffffu, odd != 0); any; any &= any - 1) {
       const int from = __ffs(any) - 1;
-      const int rr = __shfl_sync(0xffffffffu, pr, from);
-      for (unsigned which = __shfl_sync(0xffffffffu, odd, from); which; which &= which - 1)
-        redo_row<T>(a, w.s, w.b, w.head, rr, __ffs(which) - 1);
+      redo_row<T>(a, w.s, w.b, w.head, __shfl_sync(0xffffffffu, pr, from), __shfl_sync(0xffffffffu, odd, from));
     }
   }
+}
+// Joins the pieces of a unit, CTA by CTA. Many pieces belong to few rows (a long
+// decode), few to many.
+template <int T, int RU, int NT>
+__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid) {
+  const int n = w.c_last - w.c_first + 1;
+  if (T == GB_F32 || n <= 2) join_rows<T, RU, NT, T == GB_F32 ? 2 : 4, 2>(a, w, tid);
+  else if (n <= 4) join_rows<T, RU, NT, 2, 4>(a, w, tid);
+  else join_rows<T, RU, NT, 1, 8>(a, w, tid);
 }
 
 // ---- the kernel on CUDA cores (float32 pools) ------------------------------------------------
@@ -557,7 +567,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
 #pragma unroll
         for (int half = 0; half < 2; half++)
           if (any >> (16 * half) & 0xFFFFu)
-            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r, -1);
+            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r, 0xFFFFFFFFu);
       }
       continue;
     }
@@ -582,7 +592,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
     __syncthreads();
     if (arrived != (unsigned)(c_last - c_first)) continue;
     __threadfence();
-    join_pieces<GB_F32, kCR, false, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last, false}, tid);
+    join_pieces<GB_F32, kCR, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid);
     if (tid == 0) a.counter[c_first] = 0u;  // ready for the next launch
   }
 }
@@ -592,7 +602,10 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
 // tcgen05 (M = 128, float32 accumulators in tensor memory): S = Q K^T from
 // shared memory, then O += P V with P written over S in tensor memory.
 //
-// Two softmax groups of four warps, a row to a thread. In a unit of more than
+// Two softmax groups of eight warps; a row belongs to two threads, each with
+// half of a tile's columns (and of O's): with a row to a thread a group took
+// 3,000 clocks between scores and P, three times what the tensor cores take
+// for its products, and there are too few warps to fill that. In a unit of more than
 // 128 rows each group has 128 rows of its own and both use every tile; in a
 // smaller one (decoding) both have the same rows and take alternate tiles, and
 // their two results are joined like the pieces of two CTAs. Either way one
@@ -618,26 +631,28 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
 // rounding's remainder (two products with V, in S's columns), and so none of
 // that error: few rows over few outstanding positions do not average it out.
 constexpr int kTR = 256, kTT = 128;       // rows of a unit, positions of a tile
-// 12 warps: 168 registers a thread, room for a row's 128 scores (a 13th warp would leave 128)
-constexpr int kSoftWarps = 8, kLoadWarps = 3, kMmaWarp = kSoftWarps + kLoadWarps;
+constexpr int kSoftWarps = 16, kLoadWarps = 3, kMmaWarp = kSoftWarps + kLoadWarps;
 constexpr int kTN = (kMmaWarp + 1) * 32;  // threads
 constexpr float kSlack = 8.f;
 constexpr uint32_t kChunkBytes = 128 * 128;  // 128 rows of 64 elements
 constexpr int kRingBytes = 10 * kChunkBytes;
 template <int HD>
 constexpr int ring_slots() { return kRingBytes / (HD / 64 * (int)kChunkBytes); }
+constexpr int kHeader = 3072;  // tiles lie on 1024-byte boundaries behind it
 template <int HD>
-constexpr int tc_smem() { return 2048 + 2 * HD / 64 * (int)kChunkBytes + kRingBytes; }
+constexpr int tc_smem() { return kHeader + 2 * HD / 64 * (int)kChunkBytes + kRingBytes; }
 
 struct TcShared {
-  uint64_t full[10], empty[10], landed[10], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free[2], fin;
+  uint64_t full[10], empty[10], landed[10], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free, fin;
   Plan plan;
   long long warp_sums[kTN / 32];
   uint32_t tmem;
-  unsigned arrived;
-  int dead;
+  int dead, odd;
+  Unit unit[2];          // the pieces left in this CTA's places (nr = 0: none)
+  unsigned arrived[2];
+  float top[2][2][128];  // what the two threads of a row tell each other
 };
-static_assert(sizeof(TcShared) <= 1024, "shared header");
+static_assert(sizeof(TcShared) <= kHeader, "shared header");
 
 GB_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 GB_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -685,27 +700,6 @@ GB_DEV void tc_ld32(uint32_t addr, uint32_t *v) {
         "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
         "=r"(v[30]), "=r"(v[31])
       : "r"(addr)
-      : "memory");
-}
-GB_DEV void tc_ld64(uint32_t addr, uint32_t *v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-      "%28,%29,%30,%31}, [%64]; "
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,"
-      "%60,%61,%62,%63}, [%65]; "
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
-        "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
-        "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]),
-        "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]),
-        "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]), "=r"(v[50]),
-        "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]), "=r"(v[57]),
-        "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
-      : "r"(addr), "r"(addr + 32)
       : "memory");
 }
 GB_DEV void tc_st16(uint32_t addr, const uint32_t *r) {
@@ -864,21 +858,21 @@ GB_DEV uint64_t ex2_poly(uint64_t x) {
               __uint_as_float((__float_as_uint(r1) << 23) + __float_as_uint(p1)));
 }
 
-// P of this warp's rows from the scores at s_at, in their place: powers of two
-// of s * scale + shift, rounded to T (and the remainders, unless `both`); the
-// sum of a row's. CUT: columns from `rel` on are not seen. The exponential unit
-// does four a clock and scheduler, 1024 clocks for a warp's 128 columns: as long
-// as the tensor cores take for both products. So of each eight columns two go
+// P of this warp's rows from 64 columns of scores at s_at, in their place: powers
+// of two of s * scale + shift, rounded to T (and the remainders, unless BOTH);
+// the sum of a row's. CUT: columns from `rel` on are not seen. The exponential
+// unit does four a clock and scheduler: for a tile as long as the tensor cores
+// take for both products. So of each eight columns two go
 // through ex2_poly on the multiply-add units. The loops stay rolled: straight
-// code for 128 columns outgrows the schedulers' instruction caches, and fetching
+// code for a tile outgrows the schedulers' instruction caches, and fetching
 // it took as long as running it (stalls on no instruction as many as issues).
-template <int T, bool CUT>
-GB_DEV float weights(uint32_t s_at, bool both, int rel, float scale, float shift) {
+template <int T, bool CUT, bool BOTH>
+GB_DEV float weights(uint32_t s_at, int rel, float scale, float shift) {
   const uint64_t k2 = pair(scale, scale), c2 = pair(shift, shift);
   uint64_t sum[2] = {0, 0};
 #pragma unroll 1
-  for (int h = 0; h < 4; h++) {
-    uint32_t u[32], p[16];
+  for (int h = 0; h < 2; h++) {
+    uint32_t u[32], rest[16];
     tc_ld32(s_at + 32 * h, u);
 #pragma unroll
     for (int c = 0; c < 16; c++) {
@@ -897,11 +891,11 @@ GB_DEV float weights(uint32_t s_at, bool both, int rel, float scale, float shift
         e = pair(x, y);
       }
       sum[c & 1] = add2(sum[c & 1], e);
-      p[c] = pack2<T>(x, y);
-      if (!both) u[c] = pack2_rest<T>(x, y, p[c]);
+      u[c] = pack2<T>(x, y);
+      if (!BOTH) rest[c] = pack2_rest<T>(x, y, u[c]);
     }
-    tc_st16(s_at + 32 * h, p);
-    if (!both) tc_st16(s_at + 32 * h + 16, u);
+    tc_st16(s_at + 32 * h, u);
+    if (!BOTH) tc_st16(s_at + 32 * h + 16, rest);
   }
   float x, y;
   unpair(add2(sum[0], sum[1]), x, y);
@@ -912,10 +906,9 @@ template <int T, int HD, bool TMA>
 __global__ void __launch_bounds__(kTN, 1)
     attn_chunk_tc_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map) {
-  extern __shared__ uint8_t raw[];
-  uint8_t *const base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  TcShared *const sh = (TcShared *)base;
-  const uint32_t q_at = gb_smem_u32(base) + 1024;
+  extern __shared__ __align__(1024) uint8_t tc_raw[];
+  TcShared *const sh = (TcShared *)tc_raw;
+  const uint32_t q_at = gb_smem_u32(tc_raw) + kHeader;
   constexpr uint32_t kTile = HD / 64 * kChunkBytes;
   constexpr int NS = ring_slots<HD>();
   const uint32_t ring = q_at + 2 * kTile;
@@ -926,12 +919,12 @@ __global__ void __launch_bounds__(kTN, 1)
     gb_mbar_init(&sh->q_empty, 1);
     for (int g = 0; g < 2; g++) {
       gb_mbar_init(&sh->s_full[g], 1);
-      gb_mbar_init(&sh->p_full[g], 4);
+      gb_mbar_init(&sh->p_full[g], kSoftWarps / 2);
       gb_mbar_init(&sh->pv_done[g], 1);
-      gb_mbar_init(&sh->o_free[g], 4);
     }
+    gb_mbar_init(&sh->o_free, kSoftWarps);
     gb_mbar_init(&sh->fin, 1);
-    sh->dead = 0;
+    sh->dead = sh->odd = sh->unit[0].nr = sh->unit[1].nr = 0;
     gb_mbar_fence_init();
   }
   if (warp == kMmaWarp) {
@@ -1101,24 +1094,20 @@ __global__ void __launch_bounds__(kTN, 1)
           qk(1, 0, n0 + 2, true, n == 2);
         }
       }
-      // O of the last unit has been read: at a group's first P V of this one
-      const uint32_t free_parity = (pieces & 1) ^ 1;
+      bar_wait(sh, &sh->o_free, (pieces & 1) ^ 1, a.err);  // O of the last unit has been read
       for (int t = 0; t < n; t++) {
         const uint32_t v = n0 + 2 * t + 1;
         loaded(v);
         if (both) {
-          if (t == 0) bar_wait(sh, &sh->o_free[0], free_parity, a.err);
           if (t + 1 < n) loaded(v + 1);
           p_ready(0);
           pv(0, v, t == 0, true, false);
           if (t + 1 < n) qk(0, 0, v + 1, false, false);
-          if (t == 0) bar_wait(sh, &sh->o_free[1], free_parity, a.err);
           p_ready(1);
           pv(1, v, t == 0, true, true);
           if (t + 1 < n) qk(1, 1, v + 1, true, t + 2 == n);
         } else {
           const int g = t & 1;
-          if (t < 2) bar_wait(sh, &sh->o_free[g], free_parity, a.err);
           p_ready(g);
           pv(g, v, t < 2, false, true);
           if (t + 2 < n) {
@@ -1135,9 +1124,12 @@ __global__ void __launch_bounds__(kTN, 1)
     __syncwarp();
     bar_wait(sh, &sh->fin, 0, a.err, true);
   } else {
-    // ---- softmax: thread = row
-    const int g = warp >> 2, row = tid & 127;
-    const uint32_t s_at = tmem + g * 128 + ((uint32_t)(warp & 3) << 21), o_at = s_at + 256;
+    // ---- softmax: two threads to a row
+    const int g = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_at = tmem + g * 128 + 64 * half + lanes;
+    float *const my_top = &sh->top[g][half][row], *const other_top = &sh->top[g][half ^ 1][row];
+    const int pair_bar = 2 + g * 4 + (warp & 3);
+    auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
     uint32_t ns = 0;  // tiles this group has taken
     while (w.next(a)) {
       const bool both = w.nr > 128;
@@ -1152,27 +1144,29 @@ __global__ void __launch_bounds__(kTN, 1)
         bar_wait(sh, &sh->s_full[g], ns & 1, a.err);
         tc_fence_after();
         if (warp_on) {
-          // the scores are read twice, once for the maximum and once for P: all
-          // 128 in registers would spill
-          const int rel = lim - t * kTT;
-          const bool cut = __any_sync(0xffffffffu, rel < kTT);
+          // the scores are read twice, once for the maximum and once for P
+          const int rel = lim - t * kTT - 64 * half;
+          const bool cut = __any_sync(0xffffffffu, rel < 64);
           float top = -INFINITY;
 #pragma unroll 1
           for (int h = 0; h < 2; h++) {
-            uint32_t u[64];
-            float x[64];
-            tc_ld64(s_at + 64 * h, u);
+            uint32_t u[32];
+            float x[32];
+            tc_ld32(s_at + 32 * h, u);
 #pragma unroll
-            for (int c = 0; c < 64; c++) x[c] = __uint_as_float(u[c]);
+            for (int c = 0; c < 32; c++) x[c] = __uint_as_float(u[c]);
             if (cut)
 #pragma unroll
-              for (int c = 0; c < 64; c++) x[c] = 64 * h + c < rel ? x[c] : -INFINITY;
+              for (int c = 0; c < 32; c++) x[c] = 32 * h + c < rel ? x[c] : -INFINITY;
             float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int c = 4; c < 64; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+            for (int c = 4; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
             top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
-          top *= a.scale_log2;
+          // both threads of a row go by the larger maximum
+          *my_top = top;
+          pair_sync();
+          top = fmaxf(top, *other_top) * a.scale_log2;
           const bool raise = top > m + kSlack || m == -INFINITY;
           const float mn = raise ? fmaxf(m, top) : m;
           if (__any_sync(0xffffffffu, raise)) {
@@ -1181,91 +1175,141 @@ __global__ void __launch_bounds__(kTN, 1)
             if (done) {  // O is there: the last P V must have ended before it is scaled
               bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
               tc_fence_after();
-              for (int c = 0; c < hd; c += 16) {
+              for (int c = half; c < hd / 16; c += 2) {
+                const uint32_t o_at = tmem + 256 + g * 128 + lanes + 16 * c;
                 uint32_t u[16];
-                tc_ld16(o_at + c, u);
+                tc_ld16(o_at, u);
 #pragma unroll
                 for (int e = 0; e < 16; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
-                tc_st16(o_at + c, u);
+                tc_st16(o_at, u);
               }
             }
           }
           m = mn;
           const float ms = m == -INFINITY ? 0.f : m;
-          if (cut) l += weights<T, true>(s_at, both, rel, a.scale_log2, -ms);
-          else l += weights<T, false>(s_at, both, rel, a.scale_log2, -ms);
+          if (both)
+            l += cut ? weights<T, true, true>(s_at, rel, a.scale_log2, -ms)
+                     : weights<T, false, true>(s_at, rel, a.scale_log2, -ms);
+          else
+            l += cut ? weights<T, true, false>(s_at, rel, a.scale_log2, -ms)
+                     : weights<T, false, false>(s_at, rel, a.scale_log2, -ms);
           tc_wait_st();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) gb_mbar_arrive(&sh->p_full[g]);
       }
-      // ---- the unit's end: its rows out of tensor memory
+      // ---- the unit's end: its rows out of tensor memory. The threads of a row
+      // (two, or four where both groups have it) tell each other their sums,
+      // then their maxima, and take 16 columns of O in turn. Warps without rows
+      // keep step: none reports O free twice before another has once.
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       if (done) {
         bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
         tc_fence_after();
       }
-      if (whole && both) {
-        bool odd = false;
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
-        if (warp_on)
-          for (int c = 0; c < hd; c += 32) {
-            uint32_t o[32];
-            tc_ld32(o_at + c, o);
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (mine && c + e < hd) {
-                uint32_t u[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                  const float x = __uint_as_float(o[e + 2 * k]) * inv, y = __uint_as_float(o[e + 2 * k + 1]) * inv;
-                  odd |= !isfinite(x) || !isfinite(y);
-                  u[k] = pack2<T>(x, y);
-                }
-                *(uint4 *)((uint16_t *)a.out + at + c + e) = make_uint4(u[0], u[1], u[2], u[3]);
-              }
-          }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) gb_mbar_arrive(&sh->o_free[g]);
-        for (unsigned any = __ballot_sync(0xffffffffu, odd); any; any &= any - 1)
-          redo_row<T>(a, w.s, w.b, w.head, pr - lane + __ffs(any) - 1, -1);
-        continue;
+      float f0 = 1.f, f1 = 0.f;  // weights of this group's result (both), or of the two groups'
+      *my_top = l;
+      if (both) {
+        pair_sync();
+        l += *other_top;
+        pair_sync();  // read before it is written again
+      } else {
+        const int quad_bar = 10 + (warp & 3);
+        auto quad_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory"); };
+        tc_fence_before();  // both groups' products have ended
+        quad_sync();
+        tc_fence_after();
+        const float l0 = sh->top[0][0][row] + sh->top[0][1][row], l1 = sh->top[1][0][row] + sh->top[1][1][row];
+        quad_sync();
+        *my_top = m;
+        quad_sync();
+        const float m0 = sh->top[0][0][row], m1 = sh->top[1][0][row];
+        quad_sync();
+        m = fmaxf(m0, m1);
+        const float ms = m == -INFINITY ? 0.f : m;
+        f0 = ex2(m0 - ms), f1 = ex2(m1 - ms);
+        l = f0 * l0 + f1 * l1;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // the CTA's own place has been read out
-      float *const dst = part_slot<kTR>(a, blockIdx.x, whole ? 2 : w.t0 == 0);
-      const int at = g * 128 + row;  // groups with the same rows leave two results
-      if (warp_on && done)
-        for (int c = 0; c < hd; c += 32) {
-          uint32_t o[32];
-          tc_ld32(o_at + c, o);
+      if (warp_on) {
+        const bool two = !both && w.t1 - w.t0 > 1;  // group 1 has had a tile
+        const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
+        f0 *= inv, f1 *= inv;
+        bool odd = false;
+        const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
+        float *const dst = part_slot<kTR>(a, blockIdx.x, w.t0 == 0);
+        const uint32_t o_at = tmem + 256 + (both ? g * 128 : 0) + lanes;
+        for (int c = both ? half : 2 * g + half; c < hd / 16; c += both ? 2 : 4) {
+          uint32_t u[16];
+          float o[16];
+          tc_ld16(o_at + 16 * c, u);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (mine && c + e < hd)
-              *(uint4 *)(dst + ((size_t)((c + e) >> 2) * kTR + at) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 16; e++) o[e] = __uint_as_float(u[e]) * f0;
+          if (two) {
+            tc_ld16(o_at + 128 + 16 * c, u);
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
+          }
+          if (!mine) continue;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) odd |= !isfinite(o[e]);
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              *(uint4 *)((uint16_t *)a.out + at + 16 * c + e) =
+                  make_uint4(pack2<T>(o[e], o[e + 1]), pack2<T>(o[e + 2], o[e + 3]), pack2<T>(o[e + 4], o[e + 5]),
+                             pack2<T>(o[e + 6], o[e + 7]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *(float4 *)(dst + ((4 * c + e / 4) * kTR + ur) * 4) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
         }
-      if (mine) {
-        dst[kTR * kMaxHD + at] = m;
-        dst[kTR * (kMaxHD + 1) + at] = l;
+        if (!whole && mine && !half && (both || !g)) {
+          dst[kTR * kMaxHD + ur] = m;
+          dst[kTR * (kMaxHD + 1) + ur] = l;
+        }
+        if (odd) *(volatile int *)&sh->odd = 1;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) gb_mbar_arrive(&sh->o_free[g]);
-      __threadfence();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      Unit unit = {w.s, w.b, w.head, w.r0, w.nr, 0, 0, whole};
-      if (!whole) {
-        w.holders(sh->plan, &unit.c_first, &unit.c_last);
-        if (tid == 0) sh->arrived = atomicAdd(a.counter + unit.c_first, 1u);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (sh->arrived != (unsigned)(unit.c_last - unit.c_first)) continue;
-        __threadfence();
+      if (lane == 0) gb_mbar_arrive(&sh->o_free);
+      if (!whole && tid == 0) {
+        Unit u = {w.s, w.b, w.head, w.r0, w.nr, 0, 0};
+        w.holders(sh->plan, &u.c_first, &u.c_last);
+        sh->unit[w.t0 == 0] = u;
       }
-      if (both) join_pieces<T, kTR, false, kSoftWarps * 32>(a, unit, tid);
-      else join_pieces<T, kTR, true, kSoftWarps * 32>(a, unit, tid);
-      if (!whole && tid == 0) a.counter[unit.c_first] = 0u;  // ready for the next launch
+    }
+    // ---- the CTA's end: units whose last piece this CTA has left are joined, and
+    // rows with an infinity or a NaN done again (calls within the loop above cost
+    // it registers)
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+    if (tid < 2 && sh->unit[tid].nr) sh->arrived[tid] = atomicAdd(a.counter + sh->unit[tid].c_first, 1u);
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+    __threadfence();
+    for (int i = 0; i < 2; i++) {
+      const Unit u = sh->unit[i];
+      if (!u.nr || sh->arrived[i] != (unsigned)(u.c_last - u.c_first)) continue;
+      join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid);
+      if (tid == 0) a.counter[u.c_first] = 0u;  // ready for the next launch
+    }
+    if (sh->odd) {
+      w.start(a, sh->plan);
+      while (w.next(a)) {
+        if (w.t0 != 0 || w.t1 != w.nt) continue;
+        for (int r = warp; r < w.nr; r += kSoftWarps) {
+          const int pr = w.r0 + r;
+          const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+          if (4 * lane < hd) {
+            const uint2 x = __ldcg((const uint2 *)((const uint16_t *)a.out + at + 4 * lane));
+            four<T>(make_uint4(x.x, x.y, 0, 0), v);
+          }
+          if (__any_sync(0xffffffffu, !isfinite(v[0]) || !isfinite(v[1]) || !isfinite(v[2]) || !isfinite(v[3])))
+            redo_row<T>(a, w.s, w.b, w.head, pr, 0xFFFFFFFFu);
+        }
+      }
     }
   }
   tc_fence_before();

@@ -101,66 +101,85 @@ GB_DEV long long mul_div(long long x, int y, long long z) {
 }
 
 struct Plan {
-  long long total;          // the line's length
-  int ctas;                 // the CTAs it is cut for
-  long long x0, x1;         // this CTA's run of it
-  long long rem;            // x0's place within its sequence
+  long long total;   // the line's length
+  long long x0, x1;  // this CTA's run of it
+  long long rem;     // x0's place within its sequence
+  int ctas;          // the CTAs the line is cut for
+  int b;             // the sequence x0 lies in
+};
+struct PlanShared {
+  long long rem, warp_sums[32];
   int b;
 };
 
-// Inclusive sum over the block's first NT threads (a multiple of 32, all of them calling).
-template <int NT>
-GB_DEV long long block_scan(long long v, long long *warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+GB_DEV long long warp_scan(long long v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = v;
-  __syncthreads();
-  for (int w = 0; w < warp; w++) v += warp_sums[w];
   return v;
 }
 
-// Every CTA finds its run by itself: each thread counts the tiles of a
-// sequence, and the sums of all of them are scanned (a kernel of its own for
-// it would cost a launch). All NT threads call it.
+// This CTA's run of a line of `total`. A line shorter than the grid goes to as
+// many CTAs as it has tiles, so that no CTA amid a unit is without a piece.
+GB_DEV void cut_line(Plan &p) {
+  p.ctas = (int)min((long long)gridDim.x, p.total);
+  const int me = min((int)blockIdx.x, p.ctas);
+  p.x0 = p.ctas ? mul_div(p.total, me, p.ctas) : 0;
+  p.x1 = me < p.ctas ? mul_div(p.total, me + 1, p.ctas) : p.x0;
+}
+
+// Every CTA finds its run by itself (a kernel of its own for it would cost a
+// launch): the tiles of all sequences are counted and their sums scanned. Up to
+// 64 sequences each warp does it alone, with no wait for the others; more are
+// counted by the NT threads of the block together. All of them call it.
 template <int RU, int KT, int NT>
-GB_DEV void make_plan(const ChunkArgs &a, Plan *plan, long long *warp_sums) {
-  const int tid = threadIdx.x, batch = a.c.batch;
-  long long total = 0, first = 0, scan = 0;
-  for (int b0 = 0; b0 < batch; b0 += NT) {
-    const long long v = Line<RU, KT>::seq_tiles(a, b0 + tid < batch ? seq_of(a, b0 + tid) : Seq{0, 0, 0, 0});
-    const long long s = block_scan<NT>(v, warp_sums);
-    if (b0 == 0) first = v, scan = s;
-    long long sum = 0;
-    for (int w = 0; w < NT / 32; w++) sum += warp_sums[w];
-    total += sum;
-    __syncthreads();
+GB_DEV Plan make_plan(const ChunkArgs &a, PlanShared *sp) {
+  const int tid = threadIdx.x, lane = tid & 31, batch = a.c.batch;
+  const Seq none = {0, 0, 0, 0};
+  Plan p = {0, 0, 0, 0, 0, 0};
+  if (batch <= 64) {
+    const long long v0 = Line<RU, KT>::seq_tiles(a, lane < batch ? seq_of(a, lane) : none);
+    const long long v1 = batch > 32 ? Line<RU, KT>::seq_tiles(a, lane + 32 < batch ? seq_of(a, lane + 32) : none) : 0;
+    const long long s0 = warp_scan(v0), n0 = __shfl_sync(0xffffffffu, s0, 31), s1 = warp_scan(v1) + n0;
+    p.total = __shfl_sync(0xffffffffu, s1, 31);
+    cut_line(p);
+    const unsigned in0 = __ballot_sync(0xffffffffu, s0 - v0 <= p.x0 && p.x0 < s0);
+    const unsigned in1 = __ballot_sync(0xffffffffu, s1 - v1 <= p.x0 && p.x0 < s1);
+    const int at = in0 ? __ffs(in0) - 1 : in1 ? __ffs(in1) - 1 : 0;
+    p.b = in0 ? at : at + 32;
+    p.rem = p.x0 - __shfl_sync(0xffffffffu, in0 ? s0 - v0 : s1 - v1, at);
+    return p;
   }
-  // a line shorter than the grid goes to as many CTAs as it has tiles, so that no CTA amid a unit is without a piece
-  const int ctas = (int)min((long long)gridDim.x, total), me = min((int)blockIdx.x, ctas);
-  const long long x0 = ctas ? mul_div(total, me, ctas) : 0, x1 = me < ctas ? mul_div(total, me + 1, ctas) : x0;
-  long long base = 0;
-  for (int b0 = 0; b0 < batch; b0 += NT) {
-    long long v = first, s = scan;
-    if (batch > NT) {
-      v = Line<RU, KT>::seq_tiles(a, b0 + tid < batch ? seq_of(a, b0 + tid) : Seq{0, 0, 0, 0});
-      s = block_scan<NT>(v, warp_sums);
-    }
-    if (v && base + s - v <= x0 && x0 < base + s) {
-      plan->b = b0 + tid;
-      plan->rem = x0 - (base + s - v);
-    }
-    if (batch > NT) {
-      for (int w = 0; w < NT / 32; w++) base += warp_sums[w];
+  // scans of NT sequences at a time: once for the total, once to find x0
+  for (int pass = 0; pass < 2; pass++) {
+    long long base = 0;
+    for (int b0 = 0; b0 < batch; b0 += NT) {
+      const long long v = Line<RU, KT>::seq_tiles(a, b0 + tid < batch ? seq_of(a, b0 + tid) : none);
+      long long s = warp_scan(v), sum = 0;
       __syncthreads();
+      if (lane == 31) sp->warp_sums[tid >> 5] = s;
+      __syncthreads();
+      for (int w = 0; w < NT / 32; w++) {
+        if (w == tid >> 5) s += sum;
+        sum += sp->warp_sums[w];
+      }
+      if (pass && base + s - v <= p.x0 && p.x0 < base + s) {
+        sp->b = b0 + tid;
+        sp->rem = p.x0 - (base + s - v);
+      }
+      base += sum;
+    }
+    if (!pass) {
+      p.total = base;
+      cut_line(p);
     }
   }
-  if (tid == 0) plan->total = total, plan->ctas = ctas, plan->x0 = x0, plan->x1 = x1;
   __syncthreads();
+  p.b = sp->b, p.rem = sp->rem;
+  return p;
 }
 
 // A walk over the pieces of this CTA's run: a piece is a unit's tiles [t0, t1).
@@ -206,8 +225,8 @@ struct Walk {
   // The CTAs that hold pieces of the unit just returned (t0, t1).
   GB_DEV void holders(const Plan &p, int *first, int *last) const {
     const long long y0 = x - t1, y1 = y0 + nt;  // the unit's place in the line: x is where the piece ended
-    *first = (int)(((y0 + 1) * p.ctas - 1) / p.total);
-    *last = (int)((y1 * p.ctas - 1) / p.total);
+    *first = (int)mul_div((y0 + 1) * p.ctas - 1, 1, p.total);
+    *last = (int)mul_div(y1 * p.ctas - 1, 1, p.total);
   }
   GB_DEV bool next(const ChunkArgs &a) {
     if (x >= x1) return false;
@@ -270,6 +289,29 @@ GB_DEV void put4(void *out, long long i, float x, float y, float z, float w) {
   } else {
     const __nv_bfloat162 p = __floats2bfloat162_rn(x, y), r = __floats2bfloat162_rn(z, w);
     *(uint2 *)((uint16_t *)out + i) = make_uint2(*(const uint32_t *)&p, *(const uint32_t *)&r);
+  }
+}
+
+template <int T>
+GB_DEV uint32_t pack2(float x, float y) {
+  if constexpr (T == GB_F16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const uint32_t *)&h;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t *)&h;
+  }
+}
+
+// Eight results at an element index that is a multiple of 8.
+template <int T>
+GB_DEV void put8(void *out, long long i, const float *v) {
+  if constexpr (T == GB_F32) {
+    *(float4 *)((float *)out + i) = make_float4(v[0], v[1], v[2], v[3]);
+    *(float4 *)((float *)out + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *(uint4 *)((uint16_t *)out + i) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
   }
 }
 
@@ -341,74 +383,109 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
     put4<T>(a.out, row * a.ldo + hq + 4 * my4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
+GB_DEV void cp_async16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 struct Unit {
   Seq s;
   int b, head, r0, nr, c_first, c_last;
 };
-// The joined rows of a unit, the block's first NT threads calling: neighbour
-// threads take neighbour rows, each all of its row's dimensions or, with few
-// rows, every so many. KC runs of four dimensions by PB pieces are loaded
-// together.
-template <int T, int RU, int NT, int KC, int PB>
-GB_DEV void join_rows(const ChunkArgs &a, const Unit &w, int tid) {
-  const int hd = a.c.head_dim, n4 = hd / 4, n = w.c_last - w.c_first + 1;
-  int split = 1;  // threads to a row
-  while (split < 32 && 2 * split * w.nr <= NT) split *= 2;
-  for (int i0 = 0; i0 < w.nr * split; i0 += NT) {
-    const int item = i0 + tid, r = item % w.nr, sub = item / w.nr, pr = w.r0 + r;
-    unsigned odd = 0;
-    if (sub < split) {
-      const long long row = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
-      for (int q0 = sub; q0 < n4; q0 += KC * split) {
-        float m = -INFINITY, l = 0.f;
-        float4 o[KC];
-#pragma unroll
-        for (int k = 0; k < KC; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p0 = 0; p0 < n; p0 += PB) {
-          float mi[PB], li[PB];
-          float4 v[PB][KC];
-#pragma unroll
-          for (int i = 0; i < PB; i++) {
-            mi[i] = -INFINITY, li[i] = 0.f;
-            if (p0 + i < n) {
-              const int c = w.c_first + p0 + i;
-              const uint32_t p = (uint32_t)(c * kPlaces + (c == w.c_first)) * (RU * (kMaxHD + 2));  // below 2^24
-              mi[i] = __ldcg(a.part + (p + RU * kMaxHD + r)), li[i] = __ldcg(a.part + (p + RU * (kMaxHD + 1) + r));
-#pragma unroll
-              for (int k = 0; k < KC; k++)
-                if (q0 + k * split < n4)
-                  v[i][k] = __ldcg((const float4 *)(a.part + (p + ((q0 + k * split) * RU + r) * 4)));
-            }
-          }
-          float mn = m;
-#pragma unroll
-          for (int i = 0; i < PB; i++) mn = fmaxf(mn, mi[i]);
-          const float ms = mn == -INFINITY ? 0.f : mn, g = ex2(m - ms);
+
+// Joins the pieces of a unit, CTA by CTA, all NT threads of barrier 1 calling,
+// with `room` bytes of shared memory to work in. First each row's weight of
+// each piece, 2^(m_i - max) over the joined sum, several lanes to a row; then
+// the rows, a thread to every so many runs of eight dimensions, whose pieces
+// come through shared memory by asynchronous copies, as many of them on their
+// way as fit: a unit of 256 rows brings 128 KB a piece, and with loads into
+// registers each few of them cost a round trip to L2.
+template <int T, int RU, int NT>
+__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid, uint8_t *smem, int room) {
+  constexpr uint32_t kPlace = RU * (kMaxHD + 2), kStep = kPlaces * kPlace;  // floats of a place, of a CTA's places
+  // in registers: through the reference each use is a load of some 200 clocks
+  const float *const part = a.part + (uint32_t)w.c_first * kStep;  // piece i at i * kStep, the first in its second place
+  void *const out = a.out;
+  const int hd = a.c.head_dim, G = a.G, n = w.c_last - w.c_first + 1, lane = tid & 31;
+  float *const f = (float *)smem;  // [piece][row]
+  // as many rows at a time as their weights take half the room at most
+  const int most = max(1, min(w.nr, room / 2 / (4 * n)));
+  for (int r_lo = 0; r_lo < w.nr; r_lo += most) {
+    const int nr = min(most, w.nr - r_lo);
+    int log2_lanes = 0;  // lanes to a row
+    while (log2_lanes < 5 && (2 << log2_lanes) * nr <= NT) log2_lanes++;
+    const int lanes = 1 << log2_lanes, li = tid & (lanes - 1);
+    for (int r0 = 0; r0 < nr; r0 += NT >> log2_lanes) {
+      const int r = r0 + (tid >> log2_lanes);
+      float m = -INFINITY, l = 0.f;
+      if (r < nr)
+#pragma unroll 4
+        for (int i = li; i < n; i += lanes) {
+          const float *p = part + ((uint32_t)i * kStep + (i ? 0 : kPlace) + RU * kMaxHD + r_lo + r);
+          const float mi = __ldcg(p), l_i = __ldcg(p + RU), mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
+          f[i * nr + r] = mi;
+          l = l * ex2(m - ms) + l_i * ex2(mi - ms);
           m = mn;
-          l *= g;
-#pragma unroll
-          for (int k = 0; k < KC; k++) o[k].x *= g, o[k].y *= g, o[k].z *= g, o[k].w *= g;
-#pragma unroll
-          for (int i = 0; i < PB; i++) {
-            if (mi[i] == -INFINITY && li[i] == 0.f) continue;  // nothing seen there: its outputs may not be written
-            const float f = ex2(mi[i] - ms);
-            l = fmaf(f, li[i], l);
-#pragma unroll
-            for (int k = 0; k < KC; k++) {
-              o[k].x = fmaf(f, v[i][k].x, o[k].x), o[k].y = fmaf(f, v[i][k].y, o[k].y);
-              o[k].z = fmaf(f, v[i][k].z, o[k].z), o[k].w = fmaf(f, v[i][k].w, o[k].w);
+        }
+      for (int o = 1; o < lanes; o <<= 1) {
+        const float mo = __shfl_xor_sync(0xffffffffu, m, o), lo = __shfl_xor_sync(0xffffffffu, l, o);
+        const float mn = fmaxf(m, mo), ms = mn == -INFINITY ? 0.f : mn;
+        l = l * ex2(m - ms) + lo * ex2(mo - ms);
+        m = mn;
+      }
+      if (m == -INFINITY) m = 0.f;
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      if (r < nr)
+        for (int i = li; i < n; i += lanes) f[i * nr + r] = ex2(f[i * nr + r] - m) * inv;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+    const int table = (n * nr * 4 + 15) & ~15, pairs = (room - table) / (32 * NT);  // 32-byte pieces a thread holds
+    float4 *const stage = (float4 *)(smem + table) + tid;  // slots 2 k and 2 k + 1: stage[2 k * NT], + NT
+    const uint32_t stage_at = gb_smem_u32(stage);
+    const int some = min(n, pairs), each = some == n ? pairs / some : 1;  // pieces, and runs of dimensions, at a time
+    const int per = NT / nr, sub = tid / nr, r = tid - sub * nr, pr = w.r0 + r_lo + r, n8 = sub < per ? hd / 8 : 0;
+    const int token = pr / G;
+    const long long at = (long long)(w.s.q0 + token) * a.ldo + (long long)(w.head * G + pr - token * G) * hd;
+    unsigned odd = 0;
+    for (int q0 = sub; q0 < n8; q0 += each * per) {
+      const int runs = min(each, (n8 - q0 + per - 1) / per);
+      auto fetch = [&](int c8, int p0, uint32_t to) {  // pieces p0.. of a run
+        const float *p = part + ((uint32_t)p0 * kStep + (uint32_t)(2 * c8 * RU + r_lo + r) * 4);
+        const int many = min(some, n - p0);
+#pragma unroll 4
+        for (int i = 0; i < many; i++, p += kStep, to += 32 * NT) {
+          const float *from = p + (p0 + i ? 0 : kPlace);
+          cp_async16(to, from, true);
+          cp_async16(to + 16 * NT, from + RU * 4, true);
+        }
+      };
+      for (int k = 0; k < runs; k++) fetch(q0 + k * per, 0, stage_at + (uint32_t)(k * some) * 32 * NT);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int k = 0; k < runs; k++) {
+        const int c8 = q0 + k * per;
+        float o[8] = {};
+        for (int p0 = 0; p0 < n; p0 += some) {
+          if (p0) {  // more pieces than fit: the next ones
+            fetch(c8, p0, stage_at);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+          }
+          const float *g = f + p0 * nr + r;
+          const float4 *v = stage + (size_t)(k * some) * 2 * NT;
+          const int many = min(some, n - p0);
+#pragma unroll 4
+          for (int i = 0; i < many; i++, g += nr, v += 2 * NT) {
+            const float4 x = v[0], y = v[NT];
+            const float gi = *g;
+            // a weight of zero: nothing seen there, and what lies there may not have been written
+            if (gi != 0.f) {
+              o[0] = fmaf(gi, x.x, o[0]), o[1] = fmaf(gi, x.y, o[1]), o[2] = fmaf(gi, x.z, o[2]), o[3] = fmaf(gi, x.w, o[3]);
+              o[4] = fmaf(gi, y.x, o[4]), o[5] = fmaf(gi, y.y, o[5]), o[6] = fmaf(gi, y.z, o[6]), o[7] = fmaf(gi, y.w, o[7]);
             }
           }
         }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+        put8<T>(out, at + 8 * c8, o);
+        bool fine = true;
 #pragma unroll
-        for (int k = 0; k < KC; k++) {
-          const int c4 = q0 + k * split;
-          if (c4 >= n4) continue;
-          const float x = o[k].x * inv, y = o[k].y * inv, z = o[k].z * inv, u = o[k].w * inv;
-          put4<T>(a.out, row + 4 * c4, x, y, z, u);
-          if (!isfinite(x) || !isfinite(y) || !isfinite(z) || !isfinite(u)) odd |= 1u << c4;
-        }
+        for (int e = 0; e < 8; e++) fine = fine && isfinite(o[e]);
+        if (!fine) odd |= 3u << 2 * c8;
       }
     }
     __syncwarp();
@@ -416,16 +493,8 @@ GB_DEV void join_rows(const ChunkArgs &a, const Unit &w, int tid) {
       const int from = __ffs(any) - 1;
       redo_row<T>(a, w.s, w.b, w.head, __shfl_sync(0xffffffffu, pr, from), __shfl_sync(0xffffffffu, odd, from));
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");  // the room is used up
   }
-}
-// Joins the pieces of a unit, CTA by CTA. Many pieces belong to few rows (a long
-// decode), few to many.
-template <int T, int RU, int NT>
-__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid) {
-  const int n = w.c_last - w.c_first + 1;
-  if (T == GB_F32 || n <= 2) join_rows<T, RU, NT, T == GB_F32 ? 2 : 4, 2>(a, w, tid);
-  else if (n <= 4) join_rows<T, RU, NT, 2, 4>(a, w, tid);
-  else join_rows<T, RU, NT, 1, 8>(a, w, tid);
 }
 
 // ---- the kernel on CUDA cores (float32 pools) ------------------------------------------------
@@ -435,20 +504,26 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
 constexpr int kCR = 64, kCT = 64, kCN = 256, kCS = 68;  // rows, tile, threads, padded row of the transposed tiles
 
 template <int HD>
+constexpr int f32_smem() { return (2 * HD * kCS + kCT * HD) * (int)sizeof(float); }
+
+template <int HD>
 __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_constant__ ChunkArgs a) {
   extern __shared__ __align__(16) float sm[];
   float *qs = sm;                  // [HD][kCS]: q transposed
   float *ks = qs + HD * kCS;       // [HD][kCS]: k transposed; then [kCT][kCS]: p transposed
   float *vs = ks + HD * kCS;       // [kCT][HD]
+  __shared__ PlanShared plan_shared;
   __shared__ Plan plan;
-  __shared__ long long warp_sums[kCN / 32];
   __shared__ long long prow[kCT];
   __shared__ unsigned arrived;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hd = a.c.head_dim;
   static_assert(HD >= kCT, "the probabilities take the keys' place");
-  make_plan<kCR, kCT, kCN>(a, &plan, warp_sums);
   Walk<kCR, kCT> w;
-  w.start(a, plan);
+  {
+    const Plan p = make_plan<kCR, kCT, kCN>(a, &plan_shared);
+    w.start(a, p);
+    if (tid == 0) plan = p;
+  }
   while (w.next(a)) {
     // queries, zeros past the unit's rows and past head_dim
     for (int i = tid; i < kCR * (HD / 4); i += kCN) {
@@ -592,7 +667,8 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
     __syncthreads();
     if (arrived != (unsigned)(c_last - c_first)) continue;
     __threadfence();
-    join_pieces<GB_F32, kCR, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid);
+    join_pieces<GB_F32, kCR, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid, (uint8_t *)sm,
+                                  f32_smem<HD>());
     if (tid == 0) a.counter[c_first] = 0u;  // ready for the next launch
   }
 }
@@ -613,7 +689,7 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
 //
 // K and V tiles come in order K0 V0 K1 V1 ... into a ring, with the 128-byte
 // swizzle that the descriptors name. Where the page size has a divisor of at
-// least 8 in common with the tile, one warp fetches them by TMA, a box of that
+// least 8 in common with the tile, two warps fetch them by TMA, a box of that
 // many rows to a lane, from wherever its page lies; what a box brings behind
 // the sequence's end is overwritten with zeros in V (0 NaN is NaN), and does
 // not matter in K. Other page sizes go through 16-byte asynchronous copies by
@@ -644,8 +720,8 @@ constexpr int tc_smem() { return kHeader + 2 * HD / 64 * (int)kChunkBytes + kRin
 
 struct TcShared {
   uint64_t full[10], empty[10], landed[10], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free, fin;
-  Plan plan;
-  long long warp_sums[kTN / 32];
+  PlanShared plan;
+  Plan mine;  // this CTA's, for its end
   uint32_t tmem;
   int dead, odd;
   Unit unit[2];          // the pieces left in this CTA's places (nr = 0: none)
@@ -744,19 +820,17 @@ GB_DEV void bar_wait(TcShared *sh, uint64_t *bar, uint32_t parity, unsigned *err
   *(volatile unsigned *)err = GB_DEVERR_TIMEOUT;
 }
 
-GB_DEV void cp_async16(uint32_t dst, const void *src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 GB_DEV void cp_async_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(gb_smem_u32(bar)) : "memory");
 }
 
 // A warp's copies of its 32 rows of a tile: `at` is the lane's row (elements
 // from base, -1: zeros), ppr 16-byte pieces a row, several rows a pass.
-GB_DEV void load_rows(const uint16_t *base, long long at, uint32_t tile, int row0, int ppr, int lane) {
-  const int rpp = 32 / ppr, sub = lane / ppr, pc = lane - sub * ppr;
+template <int PPR>
+GB_DEV void load_rows_of(const uint16_t *base, long long at, uint32_t tile, int row0, int ppr, int lane) {
+  const int pr = PPR ? PPR : ppr, rpp = 32 / pr, sub = lane / pr, pc = lane - sub * pr;
   const uint32_t chunk = tile + (uint32_t)(pc >> 3) * kChunkBytes;
-#pragma unroll 8
+#pragma unroll
   for (int r0 = 0; r0 < 32; r0 += rpp) {
     const int r = r0 + sub;
     const long long from = __shfl_sync(0xffffffffu, at, r & 31);
@@ -766,11 +840,18 @@ GB_DEV void load_rows(const uint16_t *base, long long at, uint32_t tile, int row
     }
   }
 }
+GB_DEV void load_rows(const uint16_t *base, long long at, uint32_t tile, int row0, int ppr, int lane) {
+  if (ppr == 16) load_rows_of<16>(base, at, tile, row0, ppr, lane);  // unrolled: 40 clocks a pass otherwise
+  else if (ppr == 8) load_rows_of<8>(base, at, tile, row0, ppr, lane);
+  else load_rows_of<0>(base, at, tile, row0, ppr, lane);
+}
 
-// A unit's queries, 32 rows at a time in turn by `warps` warps; zeros past its rows.
+// A unit's queries, 32 rows at a time in turn by `warps` warps; zeros past its
+// rows, except that whole 32 rows past them are left as they are (no softmax
+// warp looks at those).
 GB_DEV void load_q(const ChunkArgs &a, const Seq &s, int u0, int nr, int head, uint32_t q_at, uint32_t tile, int lw,
                    int warps, int ppr, int lane) {
-  for (int j = lw; j < (nr > 128 ? 8 : 4); j += warps) {
+  for (int j = lw; j * 32 < nr; j += warps) {
     const int r = j * 32 + lane, pr = u0 + r;
     const long long at =
         r < nr ? (long long)(s.q0 + pr / a.G) * a.ldq + (long long)(head * a.G + pr % a.G) * a.c.head_dim : -1;
@@ -778,21 +859,16 @@ GB_DEV void load_q(const ChunkArgs &a, const Seq &s, int u0, int nr, int head, u
   }
 }
 
-template <int T>
-GB_DEV uint32_t pack2(float x, float y) {
-  if constexpr (T == GB_F16) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *(const uint32_t *)&h;
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *(const uint32_t *)&h;
-  }
-}
-
 // The rows a TMA box holds: the page size's common divisor with a tile.
 __host__ GB_DEV int box_rows(int page_size) {
   const int low = page_size & -page_size;
   return low < kTT ? low : kTT;
+}
+
+GB_DEV uint32_t elect_lane() {
+  uint32_t on;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+  return on;
 }
 
 GB_DEV void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
@@ -913,18 +989,23 @@ __global__ void __launch_bounds__(kTN, 1)
   constexpr int NS = ring_slots<HD>();
   const uint32_t ring = q_at + 2 * kTile;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.c.head_dim;
-  if (tid == 0) {
-    for (int i = 0; i < NS; i++) gb_mbar_init(&sh->full[i], TMA ? 1 : kLoadWarps * 32), gb_mbar_init(&sh->empty[i], 1), gb_mbar_init(&sh->landed[i], 1);
-    gb_mbar_init(&sh->q_full, (TMA ? 2 : kLoadWarps) * 32);
-    gb_mbar_init(&sh->q_empty, 1);
-    for (int g = 0; g < 2; g++) {
+  if (warp == 0) {
+    if (lane < NS) {
+      gb_mbar_init(&sh->full[lane], TMA ? 1 : kLoadWarps * 32);
+      gb_mbar_init(&sh->empty[lane], 1);
+      gb_mbar_init(&sh->landed[lane], 1);
+    } else if (lane < NS + 2) {
+      const int g = lane - NS;
       gb_mbar_init(&sh->s_full[g], 1);
       gb_mbar_init(&sh->p_full[g], kSoftWarps / 2);
       gb_mbar_init(&sh->pv_done[g], 1);
+    } else if (lane == 31) {
+      gb_mbar_init(&sh->q_full, (TMA ? 1 : kLoadWarps) * 32);
+      gb_mbar_init(&sh->q_empty, 1);
+      gb_mbar_init(&sh->o_free, kSoftWarps);
+      gb_mbar_init(&sh->fin, 1);
+      sh->dead = sh->odd = sh->unit[0].nr = sh->unit[1].nr = 0;
     }
-    gb_mbar_init(&sh->o_free, kSoftWarps);
-    gb_mbar_init(&sh->fin, 1);
-    sh->dead = sh->odd = sh->unit[0].nr = sh->unit[1].nr = 0;
     gb_mbar_fence_init();
   }
   if (warp == kMmaWarp) {
@@ -933,56 +1014,67 @@ __global__ void __launch_bounds__(kTN, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  const Plan plan = make_plan<kTR, kTT, kTN>(a, &sh->plan);
+  Walk<kTR, kTT> w;
+  w.start(a, plan);
+  if (tid == 0) sh->mine = plan;
   tc_fence_before();
-  make_plan<kTR, kTT, kTN>(a, &sh->plan, sh->warp_sums);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
-  Walk<kTR, kTT> w;
-  w.start(a, sh->plan);
 
-  if (TMA && warp == kSoftWarps) {
-    // ---- K and V by TMA: lane = (box of rows, 64-element column chunk)
-    const int br = box_rows(a.c.page_size), nbox = kTT / br, chunks = (hd + 63) / 64;
-    const int box = lane % nbox, chunk = lane / nbox;
+  if (TMA && warp < kSoftWarps + 2 && warp >= kSoftWarps) {
+    // ---- K (one warp) and V (another) by TMA: lane i finds box i's row, one lane
+    // issues the boxes, a 64-element column chunk each (all lanes their own took
+    // 130 clocks a box)
+    const int kv = warp - kSoftWarps, br = box_rows(a.c.page_size), box = lane & (kTT / br - 1);
+    constexpr int chunks = HD / 64;
+    const uint32_t leader = elect_lane();
+    const CUtensorMap *const map = kv ? &v_map : &k_map;
     uint32_t n = 0;
     while (w.next(a)) {
-      // the box's first row in the pool (rows of head_dim), for tile t
-      auto first_row = [&](int t) {
-        const int p = t * kTT + box * br;
-        return t < w.t1 && chunk < chunks ? pool_row(a, w.s, w.b, w.head, p, 1) : -1;
-      };
-      long long at = first_row(w.t0);
-      for (int t = w.t0; t < w.t1; t++) {
-        const long long ahead = first_row(t + 1);  // its table entry is on its way meanwhile
+      const int32_t *const table = a.c.block_table + (long long)w.b * a.c.max_pages;
+      int p = w.t0 * kTT + box * br, page = p / a.c.page_size;
+      int phys = p < w.s.cap ? table[page] : 0;
+      for (int t = w.t0; t < w.t1; t++, n += 2) {
+        const int y0 = ((phys < 0 || phys >= a.c.n_pages ? 0 : phys) * a.c.n_kv + w.head) * a.c.page_size +
+                       p - page * a.c.page_size;
+        // the next tile's table entry is on its way while this one's rows are
+        p += kTT;
+        page = p / a.c.page_size;
+        phys = t + 1 < w.t1 && p < w.s.cap ? table[page] : 0;
         const int held = min(max(w.s.cap - t * kTT, 0), kTT), boxes = (held + br - 1) / br;
-#pragma unroll
-        for (int kv = 0; kv < 2; kv++, n++) {
-          const uint32_t slot = n % NS;
-          bar_wait(sh, &sh->empty[slot], (n / NS & 1) ^ 1, a.err);
-          // V at the sequence's end goes through the warp that puts the zeros, which then reports it full
-          uint64_t *bar = kv && held < kTT ? &sh->landed[slot] : &sh->full[slot];
-          if (lane == 0) gb_mbar_expect_tx(bar, (uint32_t)(boxes * chunks * br) * 128);
-          __syncwarp();
-          if (at >= 0)
-            tma_box(ring + slot * kTile + chunk * kChunkBytes + box * br * 128, kv ? &v_map : &k_map, chunk * 64, (int)at,
-                    bar);
+        const uint32_t slot = (n + kv) % NS;
+        bar_wait(sh, &sh->empty[slot], ((n + kv) / NS & 1) ^ 1, a.err);
+        // V at the sequence's end goes through the warp that puts the zeros, which then reports it full
+        uint64_t *bar = kv && held < kTT ? &sh->landed[slot] : &sh->full[slot];
+        if (lane == 0) gb_mbar_expect_tx(bar, (uint32_t)(boxes * chunks * br) * 128);
+        __syncwarp();
+        for (int i = 0; i < boxes; i++) {
+          const int y = __shfl_sync(0xffffffffu, y0, i);
+          const uint32_t to = ring + slot * kTile + (uint32_t)(i * br) * 128;
+          if (leader) {
+            tma_box(to, map, 0, y, bar);
+            if (HD > 64) tma_box(to + kChunkBytes, map, 64, y, bar);
+          }
         }
-        at = ahead;
+        __syncwarp();
       }
     }
     // whatever was fetched has landed before the CTA ends
-    for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) bar_wait(sh, &sh->full[i % NS], i / NS & 1, a.err, true);
-  } else if (TMA && warp < kMmaWarp && warp > kSoftWarps) {
-    // ---- queries (two warps), and zeros over V behind the sequence's end (one of them)
-    const int lw = warp - kSoftWarps - 1, ppr = hd / 8;
+    for (uint32_t i = n > NS ? n - NS : 0; i < n; i++)
+      if ((i & 1) == (uint32_t)kv) bar_wait(sh, &sh->full[i % NS], i / NS & 1, a.err, true);
+  } else if (TMA && warp == kSoftWarps + 2) {
+    // ---- queries, and zeros over V behind the sequence's end
+    const int ppr = hd / 8;
     uint32_t n0 = 0, pieces = 0, phase = 0;  // bit i: parity of the next landing in slot i
     while (w.next(a)) {
       bar_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err);
-      load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, lw, 2, ppr, lane);
+      load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, 0, 1, ppr, lane);
       cp_async_arrive(&sh->q_full);
       pieces++;
       const int last = w.s.cap / kTT;  // the tile that the end lies in
-      if (lw == 0 && last >= w.t0 && last < w.t1) {
+      if (last >= w.t0 && last < w.t1) {
         const uint32_t slot = (n0 + 2 * (last - w.t0) + 1) % NS;
         bar_wait(sh, &sh->landed[slot], phase >> slot & 1, a.err);
         phase ^= 1u << slot;
@@ -1032,8 +1124,7 @@ __global__ void __launch_bounds__(kTN, 1)
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kMmaWarp) {
     // ---- the products: the warp walks and waits together, one elected lane issues
-    uint32_t leader;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
+    const uint32_t leader = elect_lane();
     const uint32_t iq = idesc_of<T>(kTT, false), iv = idesc_of<T>(hd, true);
     uint32_t n0 = 0, pieces = 0, np0 = 0, np1 = 0;  // ring position of the piece, pieces, P's taken of each group
     // S_g = Q_qt K^T, K at ring position n; `k_done`: its slot's last use; `q_done`: the queries' last use
@@ -1136,7 +1227,7 @@ __global__ void __launch_bounds__(kTN, 1)
       const int ur = (both ? g * 128 : 0) + row, pr = w.r0 + ur;
       const bool mine = ur < w.nr;
       const bool warp_on = ur - lane < w.nr;
-      // rows past the unit's are computed with zero queries and not looked at
+      // rows past the unit's in a warp of its rows have zero queries and are not looked at
       const int lim = mine ? visible(w.s, a.G, pr) : 0x7FFFFFFF;
       float m = -INFINITY, l = 0.f;
       int done = 0;
@@ -1255,10 +1346,7 @@ __global__ void __launch_bounds__(kTN, 1)
 #pragma unroll
             for (int e = 0; e < 16; e++) odd |= !isfinite(o[e]);
 #pragma unroll
-            for (int e = 0; e < 16; e += 8)
-              *(uint4 *)((uint16_t *)a.out + at + 16 * c + e) =
-                  make_uint4(pack2<T>(o[e], o[e + 1]), pack2<T>(o[e + 2], o[e + 3]), pack2<T>(o[e + 4], o[e + 5]),
-                             pack2<T>(o[e + 6], o[e + 7]));
+            for (int e = 0; e < 16; e += 8) put8<T>(a.out, at + 16 * c + e, o + e);
           } else {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
@@ -1276,7 +1364,7 @@ __global__ void __launch_bounds__(kTN, 1)
       if (lane == 0) gb_mbar_arrive(&sh->o_free);
       if (!whole && tid == 0) {
         Unit u = {w.s, w.b, w.head, w.r0, w.nr, 0, 0};
-        w.holders(sh->plan, &u.c_first, &u.c_last);
+        w.holders(sh->mine, &u.c_first, &u.c_last);
         sh->unit[w.t0 == 0] = u;
       }
     }
@@ -1291,11 +1379,12 @@ __global__ void __launch_bounds__(kTN, 1)
     for (int i = 0; i < 2; i++) {
       const Unit u = sh->unit[i];
       if (!u.nr || sh->arrived[i] != (unsigned)(u.c_last - u.c_first)) continue;
-      join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid);
+      // the tiles' room: all of them are used up
+      join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid, tc_raw + kHeader, tc_smem<HD>() - kHeader);
       if (tid == 0) a.counter[u.c_first] = 0u;  // ready for the next launch
     }
     if (sh->odd) {
-      w.start(a, sh->plan);
+      w.start(a, sh->mine);
       while (w.next(a)) {
         if (w.t0 != 0 || w.t1 != w.nt) continue;
         for (int r = warp; r < w.nr; r += kSoftWarps) {
@@ -1373,7 +1462,7 @@ int launch_16(const ChunkArgs &a, int sms, cudaStream_t st, const char *what) {
 
 template <int HD>
 int launch_f32(const ChunkArgs &a, int ctas, cudaStream_t st, const char *what) {
-  const int smem = (2 * HD * kCS + kCT * HD) * (int)sizeof(float);
+  const int smem = f32_smem<HD>();
   GB_CUDA(cudaFuncSetAttribute(attn_chunk_f32_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
   attn_chunk_f32_kernel<HD><<<(unsigned)ctas, kCN, smem, st>>>(a);
   GB_CUDA(cudaGetLastError(), what);

@@ -28,6 +28,7 @@
 
 namespace {
 
+constexpr int kCounters = 3;
 struct ChunkArgs {
   gb_paged_chunk c;
   const void *q;
@@ -36,7 +37,7 @@ struct ChunkArgs {
   int n_heads, G;
   float scale_log2;   // scale * log2(e): the softmax is taken in powers of two
   float *part;        // partial rows (part_slot)
-  unsigned *counter;  // [CTAs], zero between launches
+  unsigned *counter;  // [CTAs][kCounters], zero between launches
   unsigned *err;      // a wait ran out (host memory)
 };
 
@@ -62,7 +63,11 @@ GB_DEV Seq seq_of(const ChunkArgs &a, int b) {
 // Positions that packed row r sees.
 GB_DEV int visible(const Seq &s, int G, int r) { return max(0, min(s.cap, s.len0 + r / G + 1)); }
 
-template <int RU, int KT>
+// The line is measured in costs, so that equal runs take equal times: a tile of
+// a unit of more than RU / 2 rows costs WIDE, of a smaller one NARROW, and a
+// unit's first tile OPEN more (its queries, the first tiles' latency, its
+// rows' way out). A tile lies where it begins.
+template <int RU, int KT, int WIDE, int NARROW, int OPEN>
 struct Line {
   static GB_DEV int units(const Seq &s, int G) { return (int)(((long long)s.n * G + RU - 1) / RU); }
   // Tiles of unit u: up to the last position its last row sees; one where none is seen, so that the rows are written.
@@ -70,21 +75,25 @@ struct Line {
     const int last = (int)min((long long)s.n * G, (long long)(u + 1) * RU) - 1;
     return max(1, (visible(s, G, last) + KT - 1) / KT);
   }
-  // Tiles of the sequences of this warp's lanes, over all KV heads (no rows: none). A sequence of many units is
+  static GB_DEV int tile_cost(const Seq &s, int G, int u) {
+    return (long long)s.n * G - (long long)u * RU > RU / 2 ? WIDE : NARROW;
+  }
+  static GB_DEV int cost(const Seq &s, int G, int u) { return OPEN + tiles(s, G, u) * tile_cost(s, G, u); }
+  // Costs of the sequences of this warp's lanes, over all KV heads (no rows: none). A sequence of many units is
   // counted by the whole warp.
-  static GB_DEV long long seq_tiles(const ChunkArgs &a, const Seq &s) {
+  static GB_DEV long long seq_cost(const ChunkArgs &a, const Seq &s) {
     const int lane = threadIdx.x & 31, nu = units(s, a.G);
     long long t = 0;
-    if (nu <= 4)
-      for (int u = 0; u < nu; u++) t += tiles(s, a.G, u);
-    for (unsigned many = __ballot_sync(0xffffffffu, nu > 4); many; many &= many - 1) {
+    if (nu <= 16)
+      for (int u = 0; u < nu; u++) t += cost(s, a.G, u);
+    for (unsigned many = __ballot_sync(0xffffffffu, nu > 16); many; many &= many - 1) {
       const int from = __ffs(many) - 1;
       Seq o;
       o.q0 = 0, o.n = __shfl_sync(0xffffffffu, s.n, from), o.len0 = __shfl_sync(0xffffffffu, s.len0, from);
       o.cap = __shfl_sync(0xffffffffu, s.cap, from);
       const int no = units(o, a.G);
       long long sum = 0;
-      for (int u = lane; u < no; u += 32) sum += tiles(o, a.G, u);
+      for (int u = lane; u < no; u += 32) sum += cost(o, a.G, u);
 #pragma unroll
       for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
       if (lane == from) t = sum;
@@ -102,7 +111,7 @@ GB_DEV long long mul_div(long long x, int y, long long z) {
 
 struct Plan {
   long long total;   // the line's length
-  long long x0, x1;  // this CTA's run of it
+  long long x0, x1;  // this CTA's run of it: the tiles that begin there
   long long rem;     // x0's place within its sequence
   int ctas;          // the CTAs the line is cut for
   int b;             // the sequence x0 lies in
@@ -122,10 +131,11 @@ GB_DEV long long warp_scan(long long v) {
   return v;
 }
 
-// This CTA's run of a line of `total`. A line shorter than the grid goes to as
-// many CTAs as it has tiles, so that no CTA amid a unit is without a piece.
-GB_DEV void cut_line(Plan &p) {
-  p.ctas = (int)min((long long)gridDim.x, p.total);
+// This CTA's run of a line of `total` whose tiles cost at most `most`. A run is
+// no shorter than that, so that no CTA amid a unit is without a piece of it.
+GB_DEV void cut_line(Plan &p, int most) {
+  p.ctas = (int)min((long long)gridDim.x, (p.total + most - 1) / most);
+  while (p.ctas > 1 && p.total < (long long)p.ctas * most) p.ctas--;
   const int me = min((int)blockIdx.x, p.ctas);
   p.x0 = p.ctas ? mul_div(p.total, me, p.ctas) : 0;
   p.x1 = me < p.ctas ? mul_div(p.total, me + 1, p.ctas) : p.x0;
@@ -135,17 +145,19 @@ GB_DEV void cut_line(Plan &p) {
 // launch): the tiles of all sequences are counted and their sums scanned. Up to
 // 64 sequences each warp does it alone, with no wait for the others; more are
 // counted by the NT threads of the block together. All of them call it.
-template <int RU, int KT, int NT>
+template <int RU, int KT, int WIDE, int NARROW, int OPEN, int NT>
 GB_DEV Plan make_plan(const ChunkArgs &a, PlanShared *sp) {
+  using L = Line<RU, KT, WIDE, NARROW, OPEN>;
   const int tid = threadIdx.x, lane = tid & 31, batch = a.c.batch;
   const Seq none = {0, 0, 0, 0};
   Plan p = {0, 0, 0, 0, 0, 0};
   if (batch <= 64) {
-    const long long v0 = Line<RU, KT>::seq_tiles(a, lane < batch ? seq_of(a, lane) : none);
-    const long long v1 = batch > 32 ? Line<RU, KT>::seq_tiles(a, lane + 32 < batch ? seq_of(a, lane + 32) : none) : 0;
+    const Seq q0 = lane < batch ? seq_of(a, lane) : none, q1 = lane + 32 < batch ? seq_of(a, lane + 32) : none;
+    const bool wide = __any_sync(0xffffffffu, (long long)max(q0.n, q1.n) * a.G > RU / 2);
+    const long long v0 = L::seq_cost(a, q0), v1 = batch > 32 ? L::seq_cost(a, q1) : 0;
     const long long s0 = warp_scan(v0), n0 = __shfl_sync(0xffffffffu, s0, 31), s1 = warp_scan(v1) + n0;
     p.total = __shfl_sync(0xffffffffu, s1, 31);
-    cut_line(p);
+    cut_line(p, (wide ? WIDE : NARROW) + OPEN);
     const unsigned in0 = __ballot_sync(0xffffffffu, s0 - v0 <= p.x0 && p.x0 < s0);
     const unsigned in1 = __ballot_sync(0xffffffffu, s1 - v1 <= p.x0 && p.x0 < s1);
     const int at = in0 ? __ffs(in0) - 1 : in1 ? __ffs(in1) - 1 : 0;
@@ -157,7 +169,7 @@ GB_DEV Plan make_plan(const ChunkArgs &a, PlanShared *sp) {
   for (int pass = 0; pass < 2; pass++) {
     long long base = 0;
     for (int b0 = 0; b0 < batch; b0 += NT) {
-      const long long v = Line<RU, KT>::seq_tiles(a, b0 + tid < batch ? seq_of(a, b0 + tid) : none);
+      const long long v = L::seq_cost(a, b0 + tid < batch ? seq_of(a, b0 + tid) : none);
       long long s = warp_scan(v), sum = 0;
       __syncthreads();
       if (lane == 31) sp->warp_sums[tid >> 5] = s;
@@ -174,7 +186,7 @@ GB_DEV Plan make_plan(const ChunkArgs &a, PlanShared *sp) {
     }
     if (!pass) {
       p.total = base;
-      cut_line(p);
+      cut_line(p, WIDE + OPEN);
     }
   }
   __syncthreads();
@@ -183,71 +195,80 @@ GB_DEV Plan make_plan(const ChunkArgs &a, PlanShared *sp) {
 }
 
 // A walk over the pieces of this CTA's run: a piece is a unit's tiles [t0, t1).
-template <int RU, int KT>
+template <int RU, int KT, int WIDE, int NARROW, int OPEN>
 struct Walk {
-  long long x, x1;
-  int b, u, h, i;
+  using L = Line<RU, KT, WIDE, NARROW, OPEN>;
+  long long y, x1;  // where the unit begins; the run's end
+  int b, u, h, i;   // sequence, unit, KV head, next tile
   // the piece
   Seq s;
   int r0, nr;      // the unit's packed rows [r0, r0 + nr) of the sequence
   int head;        // its KV head
   int t0, t1, nt;  // tiles of the piece, and of the unit
+  int cost;        // of a tile
+
+  // The first tile that begins at `pos` or later (from the unit's beginning).
+  GB_DEV int tile_at(long long pos) const { return pos <= 0 ? 0 : pos <= OPEN ? 1 : (int)mul_div(pos - OPEN + cost - 1, 1, cost); }
 
   // All lanes of the warp call it: they look through the sequence's units 32 at a time.
   GB_DEV void start(const ChunkArgs &a, const Plan &p) {
-    x = p.x0, x1 = p.x1;
-    if (x >= x1) return;
+    y = p.x0, x1 = p.x1;
+    if (y >= x1) return;
     b = p.b;
     s = seq_of(a, b);
     long long rem = p.rem;
-    const int lane = threadIdx.x & 31, nu = Line<RU, KT>::units(s, a.G);
+    const int lane = threadIdx.x & 31, nu = L::units(s, a.G);
     for (u = 0;; u += 32) {
-      const int mine = u + lane < nu ? Line<RU, KT>::tiles(s, a.G, u + lane) : 0;
-      long long sum = (long long)mine * a.c.n_kv;  // with the units before it
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
+      const int mine = u + lane < nu ? L::cost(s, a.G, u + lane) : 0;
+      const long long sum = warp_scan((long long)mine * a.c.n_kv);  // with the units before it
       const unsigned past = __ballot_sync(0xffffffffu, sum > rem);
       if (past || u + 32 >= nu) {
         const int at = past ? __ffs(past) - 1 : 0;
         u += at;
-        nt = __shfl_sync(0xffffffffu, mine, at);
-        rem -= __shfl_sync(0xffffffffu, sum, at) - (long long)nt * a.c.n_kv;
+        const int c = __shfl_sync(0xffffffffu, mine, at);
+        rem -= __shfl_sync(0xffffffffu, sum, at) - (long long)c * a.c.n_kv;
+        h = (int)mul_div(rem, 1, c);
+        rem -= (long long)h * c;
         break;
       }
       rem -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    h = (int)mul_div(rem, 1, nt);
-    i = (int)(rem - (long long)h * nt);
+    y -= rem;
+    nt = L::tiles(s, a.G, u);
+    cost = L::tile_cost(s, a.G, u);
+    i = tile_at(rem);
+    if (i >= nt) leave();
   }
-  // The CTAs that hold pieces of the unit just returned (t0, t1).
-  GB_DEV void holders(const Plan &p, int *first, int *last) const {
-    const long long y0 = x - t1, y1 = y0 + nt;  // the unit's place in the line: x is where the piece ended
-    *first = (int)mul_div((y0 + 1) * p.ctas - 1, 1, p.total);
-    *last = (int)mul_div(y1 * p.ctas - 1, 1, p.total);
+  GB_DEV void leave() {
+    y += OPEN + (long long)nt * cost;
+    h++;
+    i = 0;
   }
   GB_DEV bool next(const ChunkArgs &a) {
-    if (x >= x1) return false;
+    if (y >= x1) return false;
     if (h == a.c.n_kv) {
       h = 0;
-      if (++u == Line<RU, KT>::units(s, a.G)) {
+      if (++u == L::units(s, a.G)) {
         u = 0;
         do s = seq_of(a, ++b);
-        while (s.n == 0);  // x < x1 <= total: a sequence with rows follows
+        while (s.n == 0);  // y < x1 <= total: a sequence with rows follows
       }
-      nt = Line<RU, KT>::tiles(s, a.G, u);
+      nt = L::tiles(s, a.G, u);
+      cost = L::tile_cost(s, a.G, u);
     }
     r0 = u * RU;
     nr = (int)min((long long)RU, (long long)s.n * a.G - r0);
     head = h;
     t0 = i;
-    t1 = (int)min((long long)nt, i + (x1 - x));
-    x += t1 - t0;
-    i = 0;
-    h++;
+    t1 = min(nt, tile_at(x1 - y));
+    leave();
     return true;
+  }
+  // The CTAs that hold pieces of the unit just returned.
+  GB_DEV void holders(const Plan &p, int *first, int *last) const {
+    const long long y0 = y - OPEN - (long long)nt * cost, y1 = y0 + (nt > 1 ? OPEN + (nt - 1) * (long long)cost : 0);
+    *first = (int)mul_div((y0 + 1) * p.ctas - 1, 1, p.total);
+    *last = (int)mul_div((y1 + 1) * p.ctas - 1, 1, p.total);
   }
 };
 
@@ -391,25 +412,61 @@ struct Unit {
   int b, head, r0, nr, c_first, c_last;
 };
 
-// Joins the pieces of a unit, CTA by CTA, all NT threads of barrier 1 calling,
-// with `room` bytes of shared memory to work in. First each row's weight of
+// Joins the pieces of a unit's rows [lo, hi), CTA by CTA, all NT threads of
+// barrier 1 calling, with `room` bytes of shared memory to work in. First each row's weight of
 // each piece, 2^(m_i - max) over the joined sum, several lanes to a row; then
 // the rows, a thread to every so many runs of eight dimensions, whose pieces
 // come through shared memory by asynchronous copies, as many of them on their
 // way as fit: a unit of 256 rows brings 128 KB a piece, and with loads into
 // registers each few of them cost a round trip to L2.
 template <int T, int RU, int NT>
-__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid, uint8_t *smem, int room) {
+__device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid, uint8_t *smem, int room, int lo,
+                                         int hi) {
   constexpr uint32_t kPlace = RU * (kMaxHD + 2), kStep = kPlaces * kPlace;  // floats of a place, of a CTA's places
   // in registers: through the reference each use is a load of some 200 clocks
   const float *const part = a.part + (uint32_t)w.c_first * kStep;  // piece i at i * kStep, the first in its second place
   void *const out = a.out;
-  const int hd = a.c.head_dim, G = a.G, n = w.c_last - w.c_first + 1, lane = tid & 31;
+  const int hd = a.c.head_dim, G = a.G, n = w.c_last - w.c_first + 1;
+  if (hi - lo <= NT / 32) {  // few rows, often of many pieces: a warp to a row, a lane to four dimensions
+    const int r = lo + (tid >> 5), lane = tid & 31, pr = w.r0 + r;
+    if (r >= hi) return;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float mi = -INFINITY, l_i = 0.f;
+      const int i = i0 + lane;
+      if (i < n) {
+        const float *p = part + ((uint32_t)i * kStep + (i ? 0 : kPlace) + RU * kMaxHD + r);
+        mi = __ldcg(p), l_i = __ldcg(p + RU);
+      }
+      const float mn = fmaxf(m, gb_warp_max(mi)), ms = mn == -INFINITY ? 0.f : mn, g = ex2(m - ms), e = ex2(mi - ms);
+      l = l * g + gb_warp_sum(e * l_i);
+      o.x *= g, o.y *= g, o.z *= g, o.w *= g;
+      m = mn;
+      const float4 *p = (const float4 *)(part + ((uint32_t)i0 * kStep + (uint32_t)(min(lane, hd / 4 - 1) * RU + r) * 4));
+      const int many = min(32, n - i0);
+#pragma unroll 8
+      for (int j = 0; j < many; j++) {
+        const float4 v = __ldcg(p + (j * kStep + (i0 + j ? 0 : kPlace)) / 4);
+        const float ej = __shfl_sync(0xffffffffu, e, j);
+        // a weight of zero: nothing seen there, and what lies there may not have been written
+        if (ej != 0.f) o.x = fmaf(ej, v.x, o.x), o.y = fmaf(ej, v.y, o.y), o.z = fmaf(ej, v.z, o.z), o.w = fmaf(ej, v.w, o.w);
+      }
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    const bool fine = isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w);
+    if (4 * lane < hd)
+      put4<T>(out, (long long)(w.s.q0 + pr / G) * a.ldo + (long long)(w.head * G + pr % G) * hd + 4 * lane, o.x, o.y, o.z, o.w);
+    const unsigned odd = __ballot_sync(0xffffffffu, !fine);
+    if (odd) redo_row<T>(a, w.s, w.b, w.head, pr, odd);
+    return;
+  }
   float *const f = (float *)smem;  // [piece][row]
   // as many rows at a time as their weights take half the room at most
-  const int most = max(1, min(w.nr, room / 2 / (4 * n)));
-  for (int r_lo = 0; r_lo < w.nr; r_lo += most) {
-    const int nr = min(most, w.nr - r_lo);
+  const int most = max(1, min(hi - lo, room / 2 / (4 * n)));
+  for (int r_lo = lo; r_lo < hi; r_lo += most) {
+    const int nr = min(most, hi - r_lo);
     int log2_lanes = 0;  // lanes to a row
     while (log2_lanes < 5 && (2 << log2_lanes) * nr <= NT) log2_lanes++;
     const int lanes = 1 << log2_lanes, li = tid & (lanes - 1);
@@ -518,9 +575,9 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
   __shared__ unsigned arrived;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hd = a.c.head_dim;
   static_assert(HD >= kCT, "the probabilities take the keys' place");
-  Walk<kCR, kCT> w;
+  Walk<kCR, kCT, 1, 1, 0> w;
   {
-    const Plan p = make_plan<kCR, kCT, kCN>(a, &plan_shared);
+    const Plan p = make_plan<kCR, kCT, 1, 1, 0, kCN>(a, &plan_shared);
     w.start(a, p);
     if (tid == 0) plan = p;
   }
@@ -663,13 +720,13 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
     w.holders(plan, &c_first, &c_last);
     __threadfence();
     __syncthreads();
-    if (tid == 0) arrived = atomicAdd(a.counter + c_first, 1u);
+    if (tid == 0) arrived = atomicAdd(a.counter + kCounters * c_first, 1u);
     __syncthreads();
     if (arrived != (unsigned)(c_last - c_first)) continue;
     __threadfence();
     join_pieces<GB_F32, kCR, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid, (uint8_t *)sm,
-                                  f32_smem<HD>());
-    if (tid == 0) a.counter[c_first] = 0u;  // ready for the next launch
+                                  f32_smem<HD>(), 0, w.nr);
+    if (tid == 0) a.counter[kCounters * c_first] = 0u;  // ready for the next launch
   }
 }
 
@@ -710,6 +767,7 @@ constexpr int kTR = 256, kTT = 128;       // rows of a unit, positions of a tile
 constexpr int kSoftWarps = 16, kLoadWarps = 3, kMmaWarp = kSoftWarps + kLoadWarps;
 constexpr int kTN = (kMmaWarp + 1) * 32;  // threads
 constexpr float kSlack = 8.f;
+constexpr int kSlice = 64, kPolls = 400;  // rows joined at a time; polls (of 0.1 us and more) for a unit's other holders
 constexpr uint32_t kChunkBytes = 128 * 128;  // 128 rows of 64 elements
 constexpr int kRingBytes = 10 * kChunkBytes;
 template <int HD>
@@ -725,7 +783,7 @@ struct TcShared {
   uint32_t tmem;
   int dead, odd;
   Unit unit[2];          // the pieces left in this CTA's places (nr = 0: none)
-  unsigned arrived[2];
+  int slice[2], busy[2];  // the first row to join of each; whether to come again
   float top[2][2][128];  // what the two threads of a row tell each other
 };
 static_assert(sizeof(TcShared) <= kHeader, "shared header");
@@ -1014,8 +1072,9 @@ __global__ void __launch_bounds__(kTN, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const Plan plan = make_plan<kTR, kTT, kTN>(a, &sh->plan);
-  Walk<kTR, kTT> w;
+  // a wide tile takes 4,000 clocks, a narrow one 2,200, what a piece has before and behind its tiles some 2,000
+  const Plan plan = make_plan<kTR, kTT, 4, 2, 2, kTN>(a, &sh->plan);
+  Walk<kTR, kTT, 4, 2, 2> w;
   w.start(a, plan);
   if (tid == 0) sh->mine = plan;
   tc_fence_before();
@@ -1368,21 +1427,46 @@ __global__ void __launch_bounds__(kTN, 1)
         sh->unit[w.t0 == 0] = u;
       }
     }
-    // ---- the CTA's end: units whose last piece this CTA has left are joined, and
-    // rows with an infinity or a NaN done again (calls within the loop above cost
-    // it registers)
+    // ---- the CTA's end: the joining of the units it has left pieces of, and rows
+    // with an infinity or a NaN done again (calls within the loop above cost it
+    // registers). The holders of a unit arrive at it; once all have, its rows are
+    // taken in slices by whoever is there (one CTA alone took 10 us for 256
+    // rows). Who comes early waits for the others, who end at about the same
+    // time, but not long: the last to arrive is always there to do what is left.
+    // The last to leave makes the unit's counters ready for the next launch.
+    auto all = []() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory"); };
     __threadfence();
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-    if (tid < 2 && sh->unit[tid].nr) sh->arrived[tid] = atomicAdd(a.counter + sh->unit[tid].c_first, 1u);
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-    __threadfence();
-    for (int i = 0; i < 2; i++) {
-      const Unit u = sh->unit[i];
-      if (!u.nr || sh->arrived[i] != (unsigned)(u.c_last - u.c_first)) continue;
-      // the tiles' room: all of them are used up
-      join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid, tc_raw + kHeader, tc_smem<HD>() - kHeader);
-      if (tid == 0) a.counter[u.c_first] = 0u;  // ready for the next launch
+    all();
+    const Unit *const my_unit = &sh->unit[tid & 1];  // of the first two threads
+    unsigned *const counter = a.counter + kCounters * my_unit->c_first;
+    const unsigned holders = (unsigned)(my_unit->c_last - my_unit->c_first + 1);
+    bool there = false, busy = tid < 2 && my_unit->nr;
+    if (busy) there = atomicAdd(counter, 1u) == holders - 1;
+    for (;;) {
+      if (tid < 2) {
+        for (int k = 0; busy && !there && k < kPolls; k++) {
+          there = *(volatile unsigned *)counter == holders;
+          if (!there) __nanosleep(100);
+        }
+        const int lo = busy && there ? (int)atomicAdd(counter + 1, 1u) * kSlice : my_unit->nr;
+        sh->slice[tid] = lo;
+        busy = lo + kSlice < my_unit->nr;  // there may be another
+        sh->busy[tid] = busy;
+      }
+      __threadfence();
+      all();
+      for (int i = 0; i < 2; i++) {
+        const Unit u = sh->unit[i];
+        const int lo = sh->slice[i];
+        // in the tiles' room: all of them are used up
+        if (lo < u.nr)
+          join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid, tc_raw + kHeader, tc_smem<HD>() - kHeader, lo, min(lo + kSlice, u.nr));
+      }
+      const bool more = sh->busy[0] || sh->busy[1];
+      all();
+      if (!more) break;
     }
+    if (tid < 2 && my_unit->nr && atomicAdd(counter + 2, 1u) == holders - 1) counter[0] = counter[1] = counter[2] = 0u;
     if (sh->odd) {
       w.start(a, sh->mine);
       while (w.next(a)) {
@@ -1476,7 +1560,7 @@ int launch_f32(const ChunkArgs &a, int ctas, cudaStream_t st, const char *what) 
 size_t gb_attn_chunk_part_floats(int sms) {
   return (size_t)sms * kPlaces * std::max(2 * kCR, kTR) * (kMaxHD + 2);
 }
-int gb_attn_chunk_counters(int sms) { return 2 * sms; }
+int gb_attn_chunk_counters(int sms) { return 2 * sms * kCounters; }
 
 int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale,
                         const void *out, long long ldo) {

@@ -84,60 +84,55 @@ def test_norm_and_rotation(gb):
 # ---- the line of work (gb_chunk.cu), restated ---------------------------------
 
 
-def line_pieces(seqs, G, n_kv, RU, KT, grid, cap=1 << 30):
-    """Every CTA's pieces (sequence, unit, head, t0, t1, tiles, c_first, c_last) as the kernel walks them."""
+def line_pieces(seqs, G, n_kv, RU, KT, grid, wide, narrow, opening, cap=1 << 30):
+    """Every CTA's pieces (CTA, sequence, unit, head, t0, t1, tiles, c_first, c_last) as the kernel walks them."""
     def tiles(n, kv, u):
         last = min(n * G, (u + 1) * RU) - 1
         vis = max(0, min(min(max(kv, 0), cap), max(kv, 0) - n + last // G + 1))
         return max(1, -(-vis // KT))
+
+    def cost(n, u):
+        return wide if n * G - u * RU > RU // 2 else narrow
     units = [-(-n * G // RU) for n, _ in seqs]
-    counts = [n_kv * sum(tiles(n, kv, u) for u in range(units[b])) for b, (n, kv) in enumerate(seqs)]
-    total = sum(counts)
-    ctas = min(grid, total)
+    line = [(b, u, h) for b in range(len(seqs)) for u in range(units[b]) for h in range(n_kv)]
+    begin, total = {}, 0
+    for b, u, h in line:
+        begin[b, u, h] = total
+        total += opening + tiles(*seqs[b], u) * cost(seqs[b][0], u)
+    many = len(seqs) <= 64 and all(n * G <= RU // 2 for n, _ in seqs)
+    most = (narrow if many else wide) + opening
+    ctas = min(grid, -(-total // most))
+    while ctas > 1 and total < ctas * most:
+        ctas -= 1
     got = []
     for me in range(grid):
         m = min(me, ctas)
         x0 = total * m // ctas if ctas else 0
         x1 = total * (m + 1) // ctas if m < ctas else x0
-        x = x0
-        if x >= x1:
-            continue
-        base = 0
-        for b, c in enumerate(counts):
-            if c and base <= x0 < base + c:
-                break
-            base += c
-        rem, u = x0 - base, 0
-        while rem >= tiles(*seqs[b], u) * n_kv:
-            rem -= tiles(*seqs[b], u) * n_kv
-            u += 1
-        nt = tiles(*seqs[b], u)
-        h, i = divmod(rem, nt)
-        while x < x1:
-            if h == n_kv:
-                h, u = 0, u + 1
-                if u == units[b]:
-                    u, b = 0, b + 1
-                    while seqs[b][0] == 0:
-                        b += 1
-                nt = tiles(*seqs[b], u)
-            t1 = min(nt, i + x1 - x)
-            y0 = x - i
-            got.append((me, b, u, h, i, t1, nt, ((y0 + 1) * ctas - 1) // total, ((y0 + nt) * ctas - 1) // total))
-            x += t1 - i
-            i, h = 0, h + 1
+        for b, u, h in line:
+            y, nt, c = begin[b, u, h], tiles(*seqs[b], u), cost(seqs[b][0], u)
+            if y >= x1 or y + opening + nt * c <= x0:
+                continue
+
+            def tile_at(pos):
+                return 0 if pos <= 0 else 1 if pos <= opening else -(-(pos - opening) // c)
+            t0, t1 = tile_at(x0 - y), min(nt, tile_at(x1 - y))
+            if t0 < t1:
+                last = y + (opening + (nt - 1) * c if nt > 1 else 0)
+                got.append((me, b, u, h, t0, t1, nt, ((y + 1) * ctas - 1) // total, ((last + 1) * ctas - 1) // total))
     return got, units, tiles
 
 
-@pytest.mark.parametrize("RU,KT,grid", [(64, 64, 296), (256, 128, 148), (64, 64, 3)])
-def test_every_tile_has_one_cta_and_every_unit_its_joiners(RU, KT, grid):
+@pytest.mark.parametrize("RU,KT,grid,costs", [(64, 64, 296, (1, 1, 0)), (256, 128, 148, (4, 2, 2)), (64, 64, 3, (1, 1, 0)),
+                                              (256, 128, 7, (4, 2, 2))])
+def test_every_tile_has_one_cta_and_every_unit_its_joiners(RU, KT, grid, costs):
     import random
     r = random.Random(RU + grid)
-    for _ in range(60):
+    for _ in range(40):
         seqs = [(r.choice([0, 1, 1, r.randint(1, 300)]), r.choice([0, r.randint(1, 40), r.randint(1, 6000)]))
                 for _ in range(r.choice([1, 2, 9, 70]))]
         G, n_kv = r.choice([1, 3, 4, 8, 71]), r.choice([1, 2, 8])
-        got, units, tiles = line_pieces(seqs, G, n_kv, RU, KT, grid)
+        got, units, tiles = line_pieces(seqs, G, n_kv, RU, KT, grid, *costs)
         by = {}
         slots = set()
         for me, b, u, h, t0, t1, nt, first, last in got:

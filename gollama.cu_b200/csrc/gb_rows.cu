@@ -23,7 +23,7 @@
 namespace {
 
 constexpr int kMaxHD = 256;       // head_dim
-constexpr int kMaxThreads = 512;  // threads of a CTA
+constexpr int kMaxThreads = 320;  // threads of a CTA, a task each
 
 struct RowArgs {
   const void *q, *k, *v;  // rows of n_heads / n_kv / n_kv heads (v only for the append)
@@ -34,29 +34,47 @@ struct RowArgs {
   int lph_log2;           // lanes per head (16 elements a lane)
   const float *wq, *wk, *freq;
   float eps;
-  double log2_base;
+  double log2_step;       // of the angles' ratio: -2 log2(base) / dims
   const int32_t *pos;     // without the append
+  int rows;
   gb_paged_chunk c;       // with the append
 };
 
+// Eight elements of type T: their bytes, and their values.
 template <int T>
-GB_DEV void ld8(const void *base, long long i, float *o) {
+struct Raw {
+  uint4 u[T == GB_F32 ? 2 : 1];
+};
+template <int T>
+GB_DEV Raw<T> fetch8(const void *base, long long i) {
+  Raw<T> r;
   if constexpr (T == GB_F32) {
-    const float4 x = *(const float4 *)((const float *)base + i), y = *(const float4 *)((const float *)base + i + 4);
-    o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w, o[4] = y.x, o[5] = y.y, o[6] = y.z, o[7] = y.w;
+    r.u[0] = *(const uint4 *)((const float *)base + i);
+    r.u[1] = *(const uint4 *)((const float *)base + i + 4);
   } else {
-    const uint4 u = *(const uint4 *)((const uint16_t *)base + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    r.u[0] = *(const uint4 *)((const uint16_t *)base + i);
+  }
+  return r;
+}
+template <int T>
+GB_DEV void values8(const Raw<T> &r, float *o) {
+  const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      if constexpr (T == GB_F16) {
-        o[2 * e] = gb_half_to_float((uint16_t)w[e]);
-        o[2 * e + 1] = gb_half_to_float((uint16_t)(w[e] >> 16));
-      } else {
-        o[2 * e] = __uint_as_float(w[e] << 16);
-        o[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-      }
+  for (int e = 0; e < 4; e++) {
+    if constexpr (T == GB_F32) {
+      o[e] = __uint_as_float(w[e]);
+    } else if constexpr (T == GB_F16) {
+      o[2 * e] = gb_half_to_float((uint16_t)w[e]);
+      o[2 * e + 1] = gb_half_to_float((uint16_t)(w[e] >> 16));
+    } else {
+      o[2 * e] = __uint_as_float(w[e] << 16);
+      o[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
     }
+  }
+  if constexpr (T == GB_F32) {
+    const uint32_t v[4] = {r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[4 + e] = __uint_as_float(v[e]);
   }
 }
 
@@ -102,131 +120,202 @@ GB_DEV Task task_of(const RowArgs &a, int t) {
   return k;
 }
 
-template <int TI>
-GB_DEV void task_load(const RowArgs &a, const Task &k, long long row, float *x) {
-  if (!k.on) {
-#pragma unroll
-    for (int e = 0; e < 16; e++) x[e] = 0.f;
-    return;
-  }
-  const void *p;
-  long long at;
-  if (k.head < a.nq) p = a.q, at = row * a.ldq + (long long)k.head * a.hd;
-  else if (k.head < a.nq + a.nk) p = a.k, at = row * a.ldk + (long long)(k.head - a.nq) * a.hd;
-  else p = a.v, at = row * a.ldv + (long long)(k.head - a.nq - a.nk) * a.hd;
-  ld8<TI>(p, at + k.dA, x);
-  ld8<TI>(p, at + k.dB, x + 8);
+// Where a task's elements lie in row 0, and the distance between rows.
+GB_DEV const void *task_source(const RowArgs &a, const Task &k, long long *at, long long *ld) {
+  const int h = k.head < a.nq ? k.head : k.head < a.nq + a.nk ? k.head - a.nq : k.head - a.nq - a.nk;
+  *at = (long long)h * a.hd;
+  *ld = k.head < a.nq ? a.ldq : k.head < a.nq + a.nk ? a.ldk : a.ldv;
+  return k.head < a.nq ? a.q : k.head < a.nq + a.nk ? a.k : a.v;
 }
 
-// One CTA per row; thread t takes the tasks t, t + blockDim, ... of the row's
-// heads. The first task's elements are in flight while the row's sequence is
-// looked up and the dims/2 angles are formed once for all heads.
-template <int TI, int TO, bool APPEND>
-__global__ void __launch_bounds__(kMaxThreads) head_rows_kernel(const __grid_constant__ RowArgs a) {
-  __shared__ float2 cs[kMaxHD / 2];
-  __shared__ int seq;
-  const int row = blockIdx.x, tid = threadIdx.x;
-  const int tasks = (a.nq + a.nk + a.nv) << a.lph_log2;
-  float x[16];
-  Task k = task_of(a, tid);
-  task_load<TI>(a, k, row, x);
-  long long p;
-  long long slot = 0;   // element index of the appended row in head 0 of its page
-  bool stored = false;  // the row has a place in the pools
-  if constexpr (APPEND) {
-    if (tid == 0) seq = a.c.batch;
-    __syncthreads();
-    for (int b = tid; b < a.c.batch; b += blockDim.x)
-      if (a.c.q_start[b] <= row && row < a.c.q_start[b + 1]) atomicMin(&seq, b);
-    __syncthreads();
-    const int b = seq;
-    if (b >= a.c.batch) return;  // a row of no sequence stays as it is
-    p = (long long)a.c.kv_lens[b] - a.c.q_start[b + 1] + row;
-    if (p >= 0 && p < (long long)a.c.max_pages * a.c.page_size) {
-      const int page = a.c.block_table[(long long)b * a.c.max_pages + p / a.c.page_size];
-      stored = page >= 0 && page < a.c.n_pages;
-      slot = ((long long)page * a.c.n_kv * a.c.page_size + p % a.c.page_size) * a.hd;
+// Waits until at most n of this thread's groups of copies (n known when the loop
+// over rows is unrolled) are on their way.
+GB_DEV void rows_landed(int n) {
+  if (n >= 5) asm volatile("cp.async.wait_group 5;" ::: "memory");
+  else if (n == 4) asm volatile("cp.async.wait_group 4;" ::: "memory");
+  else if (n == 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// R rows by a slice of their heads to a CTA, a thread to the same 16 elements of
+// a head in each row: all rows' elements are on their way while the rows'
+// sequences are looked up (by each warp for itself) and their R dims/2 angles
+// formed, once for all heads. With few rows R is 1, for the most CTAs. With many
+// it is 6 (3 in float32), the elements on their way to shared memory, where a
+// thread reads what it asked for: 8192 rows of 72 heads of 128 took 84 us with
+// one row to a CTA, and as long with four held in registers, of which an SM has
+// too few to keep the memory busy.
+template <int TI, int TO, bool APPEND, int R>
+__global__ void __launch_bounds__(kMaxThreads, R > 1 ? 3 : 1) head_rows_kernel(const __grid_constant__ RowArgs a) {
+  constexpr int kParts = sizeof(Raw<TI>) / 16;  // 16-byte parts of eight elements
+  __shared__ float2 cs[R][kMaxHD / 2];          // pair j of row i at [i][(j % 8) * half / 8 + j / 8]
+  extern __shared__ uint4 stage[];              // [row][part of both runs][thread]
+  const int row0 = blockIdx.x * R, tid = threadIdx.x, lane = tid & 31, half = a.dims / 2, eighth = half / 8;
+  const Task k = task_of(a, (int)(blockIdx.y * blockDim.x) + tid);
+  Raw<TI> xa = {}, xb = {};
+  long long src_at, ld;
+  const void *const src = task_source(a, k, &src_at, &ld);
+  if constexpr (R == 1) {
+    if (k.on) {
+      xa = fetch8<TI>(src, row0 * ld + src_at + k.dA);
+      xb = fetch8<TI>(src, row0 * ld + src_at + k.dB);
     }
   } else {
-    p = a.pos ? a.pos[row] : 0;
-  }
-  for (int j = tid; j < a.dims / 2; j += blockDim.x) {
-    double turns = (double)p * exp2(a.log2_base * (-2.0 * j / a.dims)) * 0.15915494309189535;  // 1 / (2 pi)
-    if (a.freq) turns /= (double)a.freq[j];
-    sincospif((float)(2.0 * (turns - rint(turns))), &cs[j].y, &cs[j].x);
-  }
-  __syncthreads();
-  for (int t = tid;;) {
-    const bool is_q = k.head < a.nq, is_v = k.head >= a.nq + a.nk;
-    const float *w = is_q ? a.wq : is_v ? nullptr : a.wk;
-    // the lanes of a head sit in one warp and agree on w, but a warp's heads may
-    // differ: the sum is formed by all lanes, and used where there is a weight
-    float ss = 0.f;
+    const uint32_t to = gb_smem_u32(stage + tid);
+    constexpr int kSize = TI == GB_F32 ? 4 : 2;
 #pragma unroll
-    for (int e = 0; e < 16; e++) ss = fmaf(x[e], x[e], ss);
-    for (int o = 1; o < (1 << a.lph_log2); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (k.on) {
-      if (w) {
-        const float r = rsqrtf(ss / (float)a.hd + a.eps);
-        float wv[16];
-        ld8<GB_F32>(w, k.dA, wv);
-        ld8<GB_F32>(w, k.dB, wv + 8);
+    for (int i = 0; i < R; i++) {
+      if (k.on && row0 + i < a.rows) {
+        const uint8_t *from = (const uint8_t *)src + ((row0 + i) * ld + src_at) * kSize;
 #pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = x[e] * r * wv[e];
-      }
-      if (k.rot) {
-        if (a.halves) {
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float2 c = cs[k.dA + e];
-            const float u = x[e], v = x[e + 8];
-            x[e] = u * c.x - v * c.y;
-            x[e + 8] = u * c.y + v * c.x;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float2 c = cs[k.dA / 2 + e];
-            const float u = x[2 * e], v = x[2 * e + 1];
-            x[2 * e] = u * c.x - v * c.y;
-            x[2 * e + 1] = u * c.y + v * c.x;
-          }
+        for (int part = 0; part < 2 * kParts; part++) {
+          const uint8_t *at = from + (part < kParts ? k.dA * kSize + part * 16 : k.dB * kSize + (part - kParts) * 16);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           to + (uint32_t)(i * 2 * kParts + part) * blockDim.x * 16),
+                       "l"(at)
+                       : "memory");
         }
       }
-      void *dst;
-      long long at;
-      if (is_q) {
-        dst = a.q_out, at = (long long)row * a.ldqo + (long long)k.head * a.hd;
-      } else if (APPEND) {
-        dst = is_v ? a.c.v_pool : a.c.k_pool;
-        const int h = k.head - a.nq - (is_v ? a.nk : 0);
-        at = slot + (long long)h * a.c.page_size * a.hd;
-      } else {
-        dst = a.k_out, at = (long long)row * a.ldko + (long long)(k.head - a.nq) * a.hd;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  // lane i knows row i: whether it belongs to a sequence, its position, and the
+  // element index of its slot in head 0 of its page (-1: none)
+  const int row = row0 + lane;
+  bool there = lane < R && row < a.rows;
+  long long p = 0, slot = -1;
+  if constexpr (APPEND) {
+    int b = -1;
+    for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
+      const bool in = b0 + lane < a.c.batch;
+      const int lo = in ? a.c.q_start[b0 + lane] : 0, hi = in ? a.c.q_start[b0 + lane + 1] : 0;
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const unsigned hit = __ballot_sync(0xffffffffu, lo <= row0 + i && row0 + i < hi);
+        if (lane == i && b < 0 && hit) b = b0 + __ffs(hit) - 1;
       }
-      if (is_q || !APPEND || stored) {
-        st8<TO>(dst, at + k.dA, x);
-        st8<TO>(dst, at + k.dB, x + 8);
+      if (__all_sync(0xffffffffu, !there || b >= 0)) break;
+    }
+    there = there && b >= 0;
+    if (there) {
+      p = (long long)a.c.kv_lens[b] - a.c.q_start[b + 1] + row;
+      if (p >= 0 && p < (long long)a.c.max_pages * a.c.page_size) {
+        const int at = (int)p, n = at / a.c.page_size, page = a.c.block_table[(long long)b * a.c.max_pages + n];
+        if (page >= 0 && page < a.c.n_pages)
+          slot = ((long long)page * a.c.n_kv * a.c.page_size + at - n * a.c.page_size) * a.hd;
       }
     }
-    t += blockDim.x;
-    if ((t & ~31) >= tasks) break;  // a whole warp leaves together
-    k = task_of(a, t);
-    task_load<TI>(a, k, row, x);
+  } else if (there && a.pos) {
+    p = a.pos[row];
   }
+  const unsigned rows_there = __ballot_sync(0xffffffffu, there);
+  for (int at0 = 0; at0 < R * half; at0 += blockDim.x) {
+    const int at = at0 + tid, i = min(at / max(half, 1), R - 1), j = at - i * half;
+    const long long pi = __shfl_sync(0xffffffffu, p, i);
+    if (at < R * half) {
+      double turns = (double)pi * exp2(a.log2_step * j) * 0.15915494309189535;  // 1 / (2 pi)
+      if (a.freq) turns /= (double)a.freq[j];
+      float2 &c = cs[i][(j & 7) * eighth + (j >> 3)];  // a warp's lanes read neighbours
+      sincospif((float)(2.0 * (turns - rint(turns))), &c.y, &c.x);
+    }
+  }
+  __syncthreads();
+  const bool is_q = k.head < a.nq, is_v = k.head >= a.nq + a.nk;
+  const float *w = is_q ? a.wq : is_v ? nullptr : a.wk;
+  const int h = is_q ? k.head : k.head - a.nq - (is_v ? a.nk : 0);
+  const int l8 = (a.halves ? k.dA : k.dA / 2) >> 3;  // the task's pairs are 8 l8 ..
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    if constexpr (R > 1) {
+      rows_landed(R - 1 - i);
+#pragma unroll
+      for (int part = 0; part < kParts; part++) {
+        xa.u[part] = stage[(i * 2 * kParts + part) * blockDim.x + tid];
+        xb.u[part] = stage[(i * 2 * kParts + kParts + part) * blockDim.x + tid];
+      }
+    }
+    float x[16];
+    values8<TI>(xa, x);
+    values8<TI>(xb, x + 8);
+    const long long slot_i = __shfl_sync(0xffffffffu, slot, i);
+    if (a.wq || a.wk) {
+      // the lanes of a head sit in one warp and agree on w, but a warp's heads may
+      // differ: the sum is formed by all lanes, and used where there is a weight
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e++) ss = fmaf(x[e], x[e], ss);
+      for (int o = 1; o < (1 << a.lph_log2); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (k.on && w) {
+        const float r = rsqrtf(ss / (float)a.hd + a.eps);
+        float wv[8];
+        values8<GB_F32>(fetch8<GB_F32>(w, k.dA), wv);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = x[e] * r * wv[e];
+        values8<GB_F32>(fetch8<GB_F32>(w, k.dB), wv);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e + 8] = x[e + 8] * r * wv[e];
+      }
+    }
+    if (!k.on || !(rows_there >> i & 1)) continue;
+    if (k.rot) {
+      if (a.halves) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float2 c = cs[i][e * eighth + l8];
+          const float u = x[e], v = x[e + 8];
+          x[e] = u * c.x - v * c.y;
+          x[e + 8] = u * c.y + v * c.x;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float2 c = cs[i][e * eighth + l8];
+          const float u = x[2 * e], v = x[2 * e + 1];
+          x[2 * e] = u * c.x - v * c.y;
+          x[2 * e + 1] = u * c.y + v * c.x;
+        }
+      }
+    }
+    void *dst;
+    long long at;
+    if (is_q) {
+      dst = a.q_out, at = (row0 + i) * a.ldqo + (long long)h * a.hd;
+    } else if (APPEND) {
+      if (slot_i < 0) continue;
+      dst = is_v ? a.c.v_pool : a.c.k_pool;
+      at = slot_i + (long long)h * a.c.page_size * a.hd;
+    } else {
+      dst = a.k_out, at = (row0 + i) * a.ldko + (long long)h * a.hd;
+    }
+    st8<TO>(dst, at + k.dA, x);
+    st8<TO>(dst, at + k.dB, x + 8);
+  }
+}
+
+template <int I, int O, bool APPEND>
+int launch_types(const RowArgs &a, cudaStream_t st, const char *what) {
+  // a task to a thread: slices of the heads beside one another
+  const int tasks = (a.nq + a.nk + a.nv) << a.lph_log2, slices = (tasks + kMaxThreads - 1) / kMaxThreads;
+  const int threads = ((tasks + slices - 1) / slices + 31) / 32 * 32;
+  // several rows to a CTA once that leaves every SM its three CTAs
+  constexpr int R = I == GB_F32 ? 3 : 6;
+  if (a.rows >= 148 * 3 * R) {
+    const int smem = R * threads * 2 * (int)sizeof(Raw<I>);
+    GB_CUDA(cudaFuncSetAttribute(head_rows_kernel<I, O, APPEND, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
+    head_rows_kernel<I, O, APPEND, R><<<dim3((unsigned)((a.rows + R - 1) / R), (unsigned)slices), (unsigned)threads, smem, st>>>(a);
+  } else {
+    head_rows_kernel<I, O, APPEND, 1><<<dim3((unsigned)a.rows, (unsigned)slices), (unsigned)threads, 0, st>>>(a);
+  }
+  GB_CUDA(cudaGetLastError(), what);
+  return GB_OK;
 }
 
 template <bool APPEND>
-int launch(const RowArgs &a, int rows, int ti, int to, cudaStream_t st, const char *what) {
-  const int tasks = (a.nq + a.nk + a.nv) << a.lph_log2;
-  const int turns = (tasks + kMaxThreads - 1) / kMaxThreads;
-  const int threads = ((tasks + turns - 1) / turns + 31) / 32 * 32;
-#define GB_ROWS(I, O)                                                              \
-  if (ti == I && to == O) {                                                        \
-    head_rows_kernel<I, O, APPEND><<<(unsigned)rows, (unsigned)threads, 0, st>>>(a); \
-    GB_CUDA(cudaGetLastError(), what);                                             \
-    return GB_OK;                                                                  \
-  }
+int launch(const RowArgs &a, int ti, int to, cudaStream_t st, const char *what) {
+#define GB_ROWS(I, O) \
+  if (ti == I && to == O) return launch_types<I, O, APPEND>(a, st, what);
   GB_ROWS(GB_F32, GB_F32)
   GB_ROWS(GB_F32, GB_F16)
   GB_ROWS(GB_F32, GB_BF16)
@@ -260,7 +349,7 @@ int common(const char *what, RowArgs &a, int nq, int nk, int nv, int hd, int row
     return gb_fail(GB_ERR_INVALID, "%s: %d query heads, %d key heads", what, nq, nk);
   if (hd < 16 || hd > kMaxHD || hd % 16)
     return gb_fail(GB_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 16 up to %d)", what, hd, kMaxHD);
-  a.nq = nq, a.nk = nk, a.nv = nv, a.hd = hd;
+  a.nq = nq, a.nk = nk, a.nv = nv, a.hd = hd, a.rows = rows;
   a.lph_log2 = 0;
   while ((16 << a.lph_log2) < hd) a.lph_log2++;
   if (rope && rope->dims) {
@@ -270,7 +359,7 @@ int common(const char *what, RowArgs &a, int nq, int nk, int nv, int hd, int row
     a.dims = rope->dims;
     a.halves = rope->halves != 0;
     a.freq = rope->freq;
-    a.log2_base = log2((double)rope->base);
+    a.log2_step = -2.0 * log2((double)rope->base) / rope->dims;
   }
   if (norm) {
     if (!(norm->eps >= 0.f)) return gb_fail(GB_ERR_INVALID, "%s: eps %g", what, norm->eps);
@@ -311,7 +400,7 @@ int gb_qk_norm_rope_launch(int typ, const void *q, long long ldq, int n_heads, c
   a.q = q, a.k = k, a.q_out = q_out, a.k_out = k_out;
   a.ldq = ldq, a.ldk = ldk, a.ldqo = ldqo, a.ldko = ldko;
   a.pos = pos;
-  return launch<false>(a, rows, typ, out_typ, st, what);
+  return launch<false>(a, typ, out_typ, st, what);
 }
 
 int gb_paged_chunk_check(const char *what, const gb_paged_chunk *c) {
@@ -347,5 +436,5 @@ int gb_rope_append_paged_launch(const gb_paged_chunk *c, int typ, const void *q,
   a.q = q, a.k = k, a.v = v, a.q_out = q_out;
   a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldqo = ldqo;
   a.c = *c;
-  return launch<true>(a, c->rows, typ, c->kv_typ, st, what);
+  return launch<true>(a, typ, c->kv_typ, st, what);
 }

@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 
@@ -554,137 +555,155 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
   }
 }
 
-// ---- the kernel on CUDA cores (float32 pools) ------------------------------------------------
-// 64 packed rows by tiles of 64 positions, 16 x 16 threads: thread (ty, tx)
-// holds the scores of rows 4 ty.. and positions 4 tx.., and of its rows'
-// outputs the dimensions 4 tx + 64 j. Everything float32.
-constexpr int kCR = 64, kCT = 64, kCN = 256, kCS = 68;  // rows, tile, threads, padded row of the transposed tiles
+// ---- the kernel on CUDA cores (float32 pools) --------------------------------
+// Up to ROWS packed rows by tiles of TILE positions, 16 x 16 threads, everything
+// float32: thread (ty, tx) has the scores of rows ty + 16 i and positions tx +
+// 16 j, and of its rows' outputs the dimensions 4 tx + 64 j. Both products read
+// four elements at a time along their sum, so keys, values and queries stay in
+// shared memory as they lie in the pools: a unit's i go up to NI = 1, 2, 4 or 8
+// by its rows, and at 8 twelve 16-byte reads feed 128 multiply-adds. K of the
+// next tile is on its way during the softmax and P V, V of it during Q K.
+constexpr int kFN = 256;  // threads
+template <int HD>
+struct F32 {
+  static constexpr int ROWS = HD == 64 ? 128 : 64, TILE = HD == 64 ? 64 : 32;
+  static constexpr int kRow = HD + 4, kP = TILE + 4;  // padded rows of Q and K, of P
+  static constexpr int kFloats = ROWS * kRow + TILE * kRow + TILE * HD + ROWS * kP;
+};
 
 template <int HD>
-constexpr int f32_smem() { return (2 * HD * kCS + kCT * HD) * (int)sizeof(float); }
-
-template <int HD>
-__global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_constant__ ChunkArgs a) {
+__global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_constant__ ChunkArgs a) {
+  using F = F32<HD>;
+  constexpr int ROWS = F::ROWS, TILE = F::TILE, kRow = F::kRow, kP = F::kP, CJ = TILE / 16;
   extern __shared__ __align__(16) float sm[];
-  float *qs = sm;                  // [HD][kCS]: q transposed
-  float *ks = qs + HD * kCS;       // [HD][kCS]: k transposed; then [kCT][kCS]: p transposed
-  float *vs = ks + HD * kCS;       // [kCT][HD]
+  float *const qs = sm, *const ks = qs + ROWS * kRow, *const vs = ks + TILE * kRow, *const ps = vs + TILE * HD;
   __shared__ PlanShared plan_shared;
   __shared__ Plan plan;
-  __shared__ long long prow[kCT];
+  __shared__ long long prow[2][TILE];
   __shared__ unsigned arrived;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hd = a.c.head_dim;
-  static_assert(HD >= kCT, "the probabilities take the keys' place");
-  Walk<kCR, kCT, 1, 1, 0> w;
+  Walk<ROWS, TILE, 1, 1, 0> w;
   {
-    const Plan p = make_plan<kCR, kCT, 1, 1, 0, kCN>(a, &plan_shared);
+    const Plan p = make_plan<ROWS, TILE, 1, 1, 0, kFN>(a, &plan_shared);
     w.start(a, p);
     if (tid == 0) plan = p;
   }
-  while (w.next(a)) {
-    // queries, zeros past the unit's rows and past head_dim
-    for (int i = tid; i < kCR * (HD / 4); i += kCN) {
-      const int r = i % kCR, d = i / kCR * 4;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (r < w.nr && d < hd) {
-        const int pr = w.r0 + r;
-        ld4<GB_F32>(a.q, (long long)(w.s.q0 + pr / a.G) * a.ldq + (long long)(w.head * a.G + pr % a.G) * hd + d, v);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; e++) qs[(d + e) * kCS + r] = v[e];
+  // a tile's rows to shared memory, `row` floats apart; zeros where there is none and past head_dim
+  auto fetch = [&](const void *pool, int t, float *to, int row) {
+    for (int i = tid; i < TILE * (HD / 4); i += kFN) {
+      const int p = i / (HD / 4), d = i % (HD / 4) * 4;
+      const long long at = prow[t & 1][p];
+      const bool there = at >= 0 && d < hd;
+      cp_async16(gb_smem_u32(to + p * row + d), (const float *)pool + (there ? at + d : 0), there);
     }
-    int lim[4];
-    float m[4], l[4], o[4][HD / 16];
+  };
+  auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  auto landed = []() { asm volatile("cp.async.wait_group 1;" ::: "memory"); };  // all but the last group
+  auto unit = [&](auto ni) {
+    constexpr int NI = decltype(ni)::value;
+    if (tid < TILE) prow[w.t0 & 1][tid] = pool_row(a, w.s, w.b, w.head, w.t0 * TILE + tid, hd);
+    for (int i = tid; i < 16 * NI * (HD / 4); i += kFN) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4, pr = w.r0 + r;
+      const bool there = r < w.nr && d < hd;
+      const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldq + (long long)(w.head * a.G + pr % a.G) * hd + d;
+      cp_async16(gb_smem_u32(qs + r * kRow + d), (const float *)a.q + (there ? at : 0), there);
+    }
+    __syncthreads();
+    fetch(a.c.k_pool, w.t0, ks, kRow);
+    commit();
+    fetch(a.c.v_pool, w.t0, vs, HD);
+    commit();
+    const int all_see = visible(w.s, a.G, w.r0);  // positions that every row sees
+    float m[NI], l[NI], o[NI][HD / 16];
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      lim[r] = 4 * ty + r < w.nr ? visible(w.s, a.G, w.r0 + 4 * ty + r) : 0;
-      m[r] = -INFINITY, l[r] = 0.f;
+    for (int i = 0; i < NI; i++) {
+      m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-      for (int d = 0; d < HD / 16; d++) o[r][d] = 0.f;
+      for (int d = 0; d < HD / 16; d++) o[i][d] = 0.f;
     }
     for (int t = w.t0; t < w.t1; t++) {
-      if (tid < kCT) prow[tid] = pool_row(a, w.s, w.b, w.head, t * kCT + tid, hd);
+      const bool more = t + 1 < w.t1;
+      if (more && tid < TILE) prow[t + 1 & 1][tid] = pool_row(a, w.s, w.b, w.head, (t + 1) * TILE + tid, hd);
+      landed();  // Q, K
       __syncthreads();
-      for (int i = tid; i < kCT * (HD / 4); i += kCN) {
-        const int p = i % kCT, d = i / kCT * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        const long long at = prow[p];
-        if (at >= 0 && d < hd) ld4<GB_F32>(a.c.k_pool, at + d, v);
+      float s[NI][CJ] = {};
+#pragma unroll 2
+      for (int d = 0; d < HD; d += 4) {
+        float4 k4[CJ];
 #pragma unroll
-        for (int e = 0; e < 4; e++) ks[(d + e) * kCS + p] = v[e];
-      }
-      for (int i = tid; i < kCT * (HD / 4); i += kCN) {
-        const int p = i / (HD / 4), d = i % (HD / 4) * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        const long long at = prow[p];
-        if (at >= 0 && d < hd) ld4<GB_F32>(a.c.v_pool, at + d, v);
-        *(float4 *)(vs + p * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
-      }
-      __syncthreads();
-      float s[4][4] = {};
-#pragma unroll 8
-      for (int d = 0; d < HD; d++) {
-        const float4 q4 = *(const float4 *)(qs + d * kCS + 4 * ty), k4 = *(const float4 *)(ks + d * kCS + 4 * tx);
-        const float qv[4] = {q4.x, q4.y, q4.z, q4.w}, kv[4] = {k4.x, k4.y, k4.z, k4.w};
+        for (int j = 0; j < CJ; j++) k4[j] = *(const float4 *)(ks + (tx + 16 * j) * kRow + d);
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int i = 0; i < NI; i++) {
+          const float4 q4 = *(const float4 *)(qs + (ty + 16 * i) * kRow + d);
 #pragma unroll
-          for (int c = 0; c < 4; c++) s[r][c] = fmaf(qv[r], kv[c], s[r][c]);
+          for (int j = 0; j < CJ; j++)
+            s[i][j] = fmaf(q4.x, k4[j].x, fmaf(q4.y, k4[j].y, fmaf(q4.z, k4[j].z, fmaf(q4.w, k4[j].w, s[i][j]))));
+        }
       }
       __syncthreads();  // the keys are used up
+      if (more) fetch(a.c.k_pool, t + 1, ks, kRow);
+      commit();
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
+      for (int i = 0; i < NI; i++) {
+        const int lim = (t + 1) * TILE <= all_see ? all_see : visible(w.s, a.G, w.r0 + ty + 16 * i);
         float mx = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          s[r][c] = t * kCT + 4 * tx + c < lim[r] ? s[r][c] * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, s[r][c]);
+        for (int j = 0; j < CJ; j++) {
+          s[i][j] = t * TILE + tx + 16 * j < lim ? s[i][j] * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
         }
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-        const float mn = fmaxf(m[r], mx), ms = mn == -INFINITY ? 0.f : mn;
-        const float f = ex2(m[r] - ms);
+        const float mn = fmaxf(m[i], mx), ms = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2(m[i] - ms);
         float sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          s[r][c] = ex2(s[r][c] - ms);
-          sum += s[r][c];
+        for (int j = 0; j < CJ; j++) {
+          s[i][j] = ex2(s[i][j] - ms);
+          sum += s[i][j];
+          ps[(ty + 16 * i) * kP + tx + 16 * j] = s[i][j];
         }
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        l[r] = fmaf(l[r], f, sum);
-        m[r] = mn;
+        l[i] = fmaf(l[i], f, sum);
+        m[i] = mn;
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++) o[r][d] *= f;
+        for (int d = 0; d < HD / 16; d++) o[i][d] *= f;
       }
-#pragma unroll
-      for (int c = 0; c < 4; c++)
-        *(float4 *)(ks + (4 * tx + c) * kCS + 4 * ty) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+      landed();  // V
       __syncthreads();
-#pragma unroll 4
-      for (int p = 0; p < kCT; p++) {
-        const float4 p4 = *(const float4 *)(ks + p * kCS + 4 * ty);
-        const float pv[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll 2
+      for (int p = 0; p < TILE; p += 4) {
+        float4 p4[NI];
 #pragma unroll
-        for (int j = 0; j < HD / 64; j++) {
-          const float4 v4 = *(const float4 *)(vs + p * HD + 64 * j + 4 * tx);
+        for (int i = 0; i < NI; i++) p4[i] = *(const float4 *)(ps + (ty + 16 * i) * kP + p);
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            o[r][4 * j] = fmaf(pv[r], v4.x, o[r][4 * j]);
-            o[r][4 * j + 1] = fmaf(pv[r], v4.y, o[r][4 * j + 1]);
-            o[r][4 * j + 2] = fmaf(pv[r], v4.z, o[r][4 * j + 2]);
-            o[r][4 * j + 3] = fmaf(pv[r], v4.w, o[r][4 * j + 3]);
+        for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float4 v4 = *(const float4 *)(vs + (p + e) * HD + 64 * j + 4 * tx);
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+              const float pe = e == 0 ? p4[i].x : e == 1 ? p4[i].y : e == 2 ? p4[i].z : p4[i].w;
+              o[i][4 * j] = fmaf(pe, v4.x, o[i][4 * j]);
+              o[i][4 * j + 1] = fmaf(pe, v4.y, o[i][4 * j + 1]);
+              o[i][4 * j + 2] = fmaf(pe, v4.z, o[i][4 * j + 2]);
+              o[i][4 * j + 3] = fmaf(pe, v4.w, o[i][4 * j + 3]);
+            }
           }
-        }
       }
-      __syncthreads();  // the tile is used up
+      __syncthreads();  // the values and weights are used up
+      if (more) fetch(a.c.v_pool, t + 1, vs, HD);
+      commit();
     }
-    if (w.t0 == 0 && w.t1 == w.nt) {
+    const bool whole = w.t0 == 0 && w.t1 == w.nt;
+    float *const dst = part_slot<ROWS>(a, blockIdx.x, w.t0 == 0);
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int pr = w.r0 + 4 * ty + r;
-        const bool on = 4 * ty + r < w.nr;
-        const float inv = l[r] != 0.f ? 1.f / l[r] : 0.f;
+    for (int i = 0; i < NI; i++) {
+      const int r = ty + 16 * i, pr = w.r0 + r;
+      const bool on = r < w.nr;
+      if (whole) {
+        const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
         const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
         bool odd = false;
 #pragma unroll
@@ -692,30 +711,33 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
           if (on && 64 * j + 4 * tx < hd) {
             float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = o[r][4 * j + k] * inv, odd |= !isfinite(v[k]);
+            for (int k = 0; k < 4; k++) v[k] = o[i][4 * j + k] * inv, odd |= !isfinite(v[k]);
             put4<GB_F32>(a.out, at + 64 * j + 4 * tx, v[0], v[1], v[2], v[3]);
           }
         const unsigned any = __ballot_sync(0xffffffffu, odd);
 #pragma unroll
         for (int half = 0; half < 2; half++)
           if (any >> (16 * half) & 0xFFFFu)
-            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + 4 * ((tid >> 5) * 2 + half) + r, 0xFFFFFFFFu);
-      }
-      continue;
-    }
-    float *dst = part_slot<kCR>(a, blockIdx.x, w.t0 == 0);
+            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + (tid >> 5) * 2 + half + 16 * i, 0xFFFFFFFFu);
+      } else if (on) {
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      if (4 * ty + r >= w.nr) continue;
-#pragma unroll
-      for (int j = 0; j < HD / 64; j++)
-        *(float4 *)(dst + ((size_t)(16 * j + tx) * kCR + 4 * ty + r) * 4) =
-            make_float4(o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]);
-      if (tx == 0) {
-        dst[kCR * kMaxHD + 4 * ty + r] = m[r];
-        dst[kCR * (kMaxHD + 1) + 4 * ty + r] = l[r];
+        for (int j = 0; j < HD / 64; j++)
+          *(float4 *)(dst + ((16 * j + tx) * ROWS + r) * 4) =
+              make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
+        if (tx == 0) {
+          dst[ROWS * kMaxHD + r] = m[i];
+          dst[ROWS * (kMaxHD + 1) + r] = l[i];
+        }
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // the empty groups
+  };
+  while (w.next(a)) {
+    if (w.nr <= 16) unit(std::integral_constant<int, 1>());
+    else if (w.nr <= 32) unit(std::integral_constant<int, 2>());
+    else if (w.nr <= 64 || ROWS == 64) unit(std::integral_constant<int, 4>());
+    else unit(std::integral_constant<int, ROWS / 16>());
+    if (w.t0 == 0 && w.t1 == w.nt) continue;
     int c_first, c_last;
     w.holders(plan, &c_first, &c_last);
     __threadfence();
@@ -724,8 +746,9 @@ __global__ void __launch_bounds__(kCN, 2) attn_chunk_f32_kernel(const __grid_con
     __syncthreads();
     if (arrived != (unsigned)(c_last - c_first)) continue;
     __threadfence();
-    join_pieces<GB_F32, kCR, kCN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid, (uint8_t *)sm,
-                                  f32_smem<HD>(), 0, w.nr);
+    join_pieces<GB_F32, ROWS, kFN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid, (uint8_t *)sm,
+                                   F::kFloats * (int)sizeof(float), 0, w.nr);
+    __syncthreads();
     if (tid == 0) a.counter[kCounters * c_first] = 0u;  // ready for the next launch
   }
 }
@@ -965,66 +988,30 @@ GB_DEV uint64_t add2(uint64_t x, uint64_t y) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
   return r;
 }
-GB_DEV float max_nan(float x, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
-}
-// 2^x of a pair without the exponential unit: x = n + f with n whole and f in
-// [-1/2, 1/2] (the sum with 1.5 2^23 leaves n in the low bits), 2^f by the
-// polynomial of degree 4 of least relative error there (2.7e-6, a ninetieth of
-// binary16's half step), n added to the exponent. Below -126 it stays there; of
-// a NaN it makes the largest number, an infinity in P: the row is done again.
-GB_DEV uint64_t ex2_poly(uint64_t x) {
-  float x0, x1, r0, r1, p0, p1;
-  unpair(x, x0, x1);
-  const uint64_t t = pair(max_nan(x0, -126.f), max_nan(x1, -126.f));
-  const uint64_t r = add2(t, pair(12582912.f, 12582912.f)), n = add2(r, pair(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pair(-1.f, -1.f), t);
-  uint64_t p = pair(0x1.3997b4p-7f, 0x1.3997b4p-7f);
-  p = fma2(p, f, pair(0x1.ca143cp-5f, 0x1.ca143cp-5f));
-  p = fma2(p, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-  p = fma2(p, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-  p = fma2(p, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  unpair(r, r0, r1);
-  unpair(p, p0, p1);
-  return pair(__uint_as_float((__float_as_uint(r0) << 23) + __float_as_uint(p0)),
-              __uint_as_float((__float_as_uint(r1) << 23) + __float_as_uint(p1)));
-}
-
 // P of this warp's rows from 64 columns of scores at s_at, in their place: powers
 // of two of s * scale + shift, rounded to T (and the remainders, unless BOTH);
-// the sum of a row's. CUT: columns from `rel` on are not seen. The exponential
-// unit does four a clock and scheduler: for a tile as long as the tensor cores
-// take for both products. So of each eight columns two go
-// through ex2_poly on the multiply-add units. The loops stay rolled: straight
-// code for a tile outgrows the schedulers' instruction caches, and fetching
-// it took as long as running it (stalls on no instruction as many as issues).
-template <int T, bool CUT, bool BOTH>
-GB_DEV float weights(uint32_t s_at, int rel, float scale, float shift) {
+// the sum of a row's. With `cut`, columns from `rel` on are not seen. The exponential unit's four a clock and
+// scheduler do not bound it: with a quarter of the powers formed by a polynomial
+// on the multiply-add units it took as long. The loop stays rolled: straight code
+// for a tile outgrows the schedulers' instruction caches, and fetching it took as
+// long as running it (stalls on no instruction as many as issues).
+template <int T, bool BOTH>
+GB_DEV float weights(uint32_t s_at, int rel, bool cut, float scale, float shift) {
   const uint64_t k2 = pair(scale, scale), c2 = pair(shift, shift);
   uint64_t sum[2] = {0, 0};
 #pragma unroll 1
   for (int h = 0; h < 2; h++) {
     uint32_t u[32], rest[16];
     tc_ld32(s_at + 32 * h, u);
+    if (cut)
+#pragma unroll
+      for (int c = 0; c < 32; c++) u[c] = 32 * h + c < rel ? u[c] : 0xFF800000u;  // -infinity
 #pragma unroll
     for (int c = 0; c < 16; c++) {
-      float x = __uint_as_float(u[2 * c]), y = __uint_as_float(u[2 * c + 1]);
-      if (CUT) {
-        x = 32 * h + 2 * c < rel ? x : -INFINITY;
-        y = 32 * h + 2 * c + 1 < rel ? y : -INFINITY;
-      }
-      uint64_t e = fma2(pair(x, y), k2, c2);
-      if (!CUT && c % 4 == 3) {
-        e = ex2_poly(e);
-        unpair(e, x, y);
-      } else {
-        unpair(e, x, y);
-        x = ex2(x), y = ex2(y);
-        e = pair(x, y);
-      }
-      sum[c & 1] = add2(sum[c & 1], e);
+      float x, y;
+      unpair(fma2(pair(__uint_as_float(u[2 * c]), __uint_as_float(u[2 * c + 1])), k2, c2), x, y);
+      x = ex2(x), y = ex2(y);
+      sum[c & 1] = add2(sum[c & 1], pair(x, y));
       u[c] = pack2<T>(x, y);
       if (!BOTH) rest[c] = pack2_rest<T>(x, y, u[c]);
     }
@@ -1073,8 +1060,8 @@ __global__ void __launch_bounds__(kTN, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // a wide tile takes 4,000 clocks, a narrow one 2,200, what a piece has before and behind its tiles some 2,000
-  const Plan plan = make_plan<kTR, kTT, 4, 2, 2, kTN>(a, &sh->plan);
-  Walk<kTR, kTT, 4, 2, 2> w;
+  const Plan plan = make_plan<kTR, kTT, 4, 2, 4, kTN>(a, &sh->plan);
+  Walk<kTR, kTT, 4, 2, 4> w;
   w.start(a, plan);
   if (tid == 0) sh->mine = plan;
   tc_fence_before();
@@ -1294,23 +1281,23 @@ __global__ void __launch_bounds__(kTN, 1)
         bar_wait(sh, &sh->s_full[g], ns & 1, a.err);
         tc_fence_after();
         if (warp_on) {
-          // the scores are read twice, once for the maximum and once for P
+          // the scores are read twice, once for the maximum and once for P: kept in
+          // registers they spilled
           const int rel = lim - t * kTT - 64 * half;
           const bool cut = __any_sync(0xffffffffu, rel < 64);
           float top = -INFINITY;
 #pragma unroll 1
           for (int h = 0; h < 2; h++) {
             uint32_t u[32];
-            float x[32];
             tc_ld32(s_at + 32 * h, u);
-#pragma unroll
-            for (int c = 0; c < 32; c++) x[c] = __uint_as_float(u[c]);
             if (cut)
 #pragma unroll
-              for (int c = 0; c < 32; c++) x[c] = 32 * h + c < rel ? x[c] : -INFINITY;
-            float mx[4] = {x[0], x[1], x[2], x[3]};
+              for (int c = 0; c < 32; c++) u[c] = 32 * h + c < rel ? u[c] : 0xFF800000u;  // -infinity
+            float mx[4];
 #pragma unroll
-            for (int c = 4; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+            for (int c = 0; c < 4; c++) mx[c] = __uint_as_float(u[c]);
+#pragma unroll
+            for (int c = 4; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(u[c]));
             top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
           // both threads of a row go by the larger maximum
@@ -1337,12 +1324,8 @@ __global__ void __launch_bounds__(kTN, 1)
           }
           m = mn;
           const float ms = m == -INFINITY ? 0.f : m;
-          if (both)
-            l += cut ? weights<T, true, true>(s_at, rel, a.scale_log2, -ms)
-                     : weights<T, false, true>(s_at, rel, a.scale_log2, -ms);
-          else
-            l += cut ? weights<T, true, false>(s_at, rel, a.scale_log2, -ms)
-                     : weights<T, false, false>(s_at, rel, a.scale_log2, -ms);
+          l += both ? weights<T, true>(s_at, rel, cut, a.scale_log2, -ms)
+                    : weights<T, false>(s_at, rel, cut, a.scale_log2, -ms);
           tc_wait_st();
         }
         tc_fence_before();
@@ -1546,9 +1529,9 @@ int launch_16(const ChunkArgs &a, int sms, cudaStream_t st, const char *what) {
 
 template <int HD>
 int launch_f32(const ChunkArgs &a, int ctas, cudaStream_t st, const char *what) {
-  const int smem = f32_smem<HD>();
+  constexpr int smem = F32<HD>::kFloats * (int)sizeof(float);
   GB_CUDA(cudaFuncSetAttribute(attn_chunk_f32_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
-  attn_chunk_f32_kernel<HD><<<(unsigned)ctas, kCN, smem, st>>>(a);
+  attn_chunk_f32_kernel<HD><<<(unsigned)ctas, kFN, smem, st>>>(a);
   GB_CUDA(cudaGetLastError(), what);
   return GB_OK;
 }
@@ -1558,7 +1541,7 @@ int launch_f32(const ChunkArgs &a, int ctas, cudaStream_t st, const char *what) 
 // Floats of partial rows and number of counters of a launch on `sms` SMs: two
 // CTAs an SM in float32, one on the tensor cores.
 size_t gb_attn_chunk_part_floats(int sms) {
-  return (size_t)sms * kPlaces * std::max(2 * kCR, kTR) * (kMaxHD + 2);
+  return (size_t)sms * kPlaces * std::max(2 * F32<64>::ROWS, kTR) * (kMaxHD + 2);
 }
 int gb_attn_chunk_counters(int sms) { return 2 * sms * kCounters; }
 

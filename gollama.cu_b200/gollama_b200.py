@@ -89,26 +89,27 @@ class PagedChunk(C.Structure):
                [(n, C.c_void_p) for n in ("q_start", "kv_lens", "block_table", "k_pool", "v_pool")]
 
 
+def _kept(params, *buffers):
+    """The buffers a description names live as long as it does; its address is taken once."""
+    params._keep, params._at = buffers, C.addressof(params)
+    return params
+
+
 def rope(base: float, dims: int, halves: bool = False, freq=None) -> RopeParams:
-    r = RopeParams(base, dims, int(halves), _ptr(freq))
-    r._keep = (freq,)  # the buffers it names live as long as it does
-    return r
+    return _kept(RopeParams(base, dims, int(halves), _ptr(freq)), freq)
 
 
 def qk_norm(wq, wk, eps: float) -> QkNormParams:
-    r = QkNormParams(_ptr(wq), _ptr(wk), eps)
-    r._keep = (wq, wk)
-    return r
+    return _kept(QkNormParams(_ptr(wq), _ptr(wk), eps), wq, wk)
 
 
 def paged_chunk(rows, batch, q_start, kv_lens, block_table, max_pages, n_pages, page_size, n_kv, head_dim, kv_typ,
                 k_pool, v_pool) -> PagedChunk:
     """The description gb_gpu_rope_append_paged and gb_gpu_attn_chunk_paged share; a program keeps one while its
     buffers stay in place and rewrites their contents from step to step."""
-    r = PagedChunk(rows, batch, max_pages, n_pages, page_size, n_kv, head_dim, kv_typ, _ptr(q_start), _ptr(kv_lens),
-                   _ptr(block_table), _ptr(k_pool), _ptr(v_pool))
-    r._keep = (q_start, kv_lens, block_table, k_pool, v_pool)
-    return r
+    return _kept(PagedChunk(rows, batch, max_pages, n_pages, page_size, n_kv, head_dim, kv_typ, _ptr(q_start),
+                            _ptr(kv_lens), _ptr(block_table), _ptr(k_pool), _ptr(v_pool)),
+                 q_start, kv_lens, block_table, k_pool, v_pool)
 
 
 _lib = None
@@ -200,25 +201,24 @@ def _check(rc: int) -> None:
 
 
 def _ptr(x) -> int | None:
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or type(x) is int:
         return x
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
+    if isinstance(x, int):
+        return x
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot pass {type(x)} as a pointer")
 
 
 def _ref(x):
-    return None if x is None else C.byref(x)
+    """Address of a description structure (None: a null pointer)."""
+    return None if x is None else getattr(x, "_at", None) or C.addressof(x)
 
 
 def _stream(s) -> int | None:
-    if s is None:
-        return None
-    if isinstance(s, int):
+    if s is None or isinstance(s, int):
         return s
     return s.cuda_stream  # torch.cuda.Stream
 

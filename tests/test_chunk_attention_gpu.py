@@ -262,3 +262,70 @@ def test_long_cache_offsets(gb, kernels, cuda):
     call(gb, kernels, B, q, 32, 0.09, b)
     torch.cuda.synchronize()
     assert torch.equal(a, b)
+
+
+def test_two_handles_on_two_streams(gb, cuda):
+    # a handle for each stream: calls that overlap on the GPU do not share a workspace
+    batches = [Batch([(1, 3000), (1, 77)], 2, 64, 16, "f16", 140), Batch([(200, 900)], 2, 64, 16, "f16", 141)]
+    ks, outs, wants = [gb.Kernels(0), gb.Kernels(0)], [], []
+    try:
+        qs = [torch.randn((B.rows, 8 * 64), generator=torch.Generator().manual_seed(i)).half().cuda()
+              for i, B in enumerate(batches)]
+        for B, q, k in zip(batches, qs, ks):
+            out = torch.zeros_like(q)
+            call(gb, k, B, q, 8, 0.125, out)
+            torch.cuda.synchronize()
+            wants.append(out.clone())
+            outs.append(out.zero_())
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for B, q, k, o, st in zip(batches, qs, ks, outs, streams):
+                call(gb, k, B, q, 8, 0.125, o, stream=st)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+    finally:
+        for k in ks:
+            k.close()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,n", [(1, 127), (1, 128), (1, 129), (1, 255), (1, 256), (1, 257), (2, 64), (2, 65),
+                                     (16, 1), (16, 8), (128, 1), (129, 1), (300, 1)])
+def test_rows_around_a_units_borders(gb, kernels, cuda, typ, heads, n):
+    # one KV head: `heads` packed rows for each new row, around 128 and 256 of them
+    run(gb, kernels, [(n, n + 170), (n, n)], heads, 1, 32, 16, typ, 150)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page", [1, 8, 16, 24, 100, 128, 192])
+def test_page_sizes_and_ends_within_a_tile(gb, kernels, cuda, typ, page):
+    run(gb, kernels, [(1, 127), (1, 128), (1, 129), (3, 255), (3, 257), (1, 1), (40, 300)], 4, 2, 64, page, typ, 160,
+        spoil=True)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_nothing_to_do(gb, kernels, cuda, typ):
+    B = Batch([(2, 20)], 2, 64, 16, typ, 170)
+    q = torch.zeros((B.rows, 4 * 64), dtype=DT[typ], device="cuda")
+    out = torch.full_like(q, 3)
+    c = B.chunk(gb)
+    for rows, batch in ((0, 1), (2, 0)):
+        c.rows, c.batch = rows, batch
+        kernels.attn_chunk_paged(c, q, 256, 4, 0.125, out, 256)
+        kernels.rope_append_paged(c, getattr(gb, typ.upper()), None, 0, 0, q, 256, q, 256, None, None, 0)
+    torch.cuda.synchronize()
+    assert (out == 3).all()
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+def test_an_infinite_key_shows(gb, kernels, cuda, typ):
+    # an infinite score makes the rows that see it NaN, as inf - inf does, and no other row
+    B = Batch([(30, 400), (4, 90)], 2, 64, 16, typ, 180)
+    q = torch.ones((B.rows, 4 * 64), dtype=DT[typ], device="cuda")
+    pages, slot = B.slots(0, 10, 11)
+    B.k[pages, :, slot] = float("inf")
+    out = torch.zeros_like(q)
+    call(gb, kernels, B, q, 4, 0.125, out)
+    torch.cuda.synchronize()
+    assert out[:30].isnan().all() and out[30:].isfinite().all()

@@ -790,7 +790,7 @@ constexpr int kTR = 256, kTT = 128;       // rows of a unit, positions of a tile
 constexpr int kSoftWarps = 16, kLoadWarps = 3, kMmaWarp = kSoftWarps + kLoadWarps;
 constexpr int kTN = (kMmaWarp + 1) * 32;  // threads
 constexpr float kSlack = 8.f;
-constexpr int kSlice = 64, kPolls = 400;  // rows joined at a time; polls (of 0.1 us and more) for a unit's other holders
+constexpr int kSlice = 64, kPolls = 64;  // rows joined at a time; polls (some 0.8 us) for a unit's other holders
 constexpr uint32_t kChunkBytes = 128 * 128;  // 128 rows of 64 elements
 constexpr int kRingBytes = 10 * kChunkBytes;
 template <int HD>

@@ -232,8 +232,9 @@ __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 3 : 1) head_rows_kernel(c
       rows_landed(R - 1 - i);
 #pragma unroll
       for (int part = 0; part < kParts; part++) {
-        xa.u[part] = stage[(i * 2 * kParts + part) * blockDim.x + tid];
-        xb.u[part] = stage[(i * 2 * kParts + kParts + part) * blockDim.x + tid];
+        // lanes past head_dim asked for nothing and add nothing to their head's sum
+        xa.u[part] = k.on ? stage[(i * 2 * kParts + part) * blockDim.x + tid] : make_uint4(0, 0, 0, 0);
+        xb.u[part] = k.on ? stage[(i * 2 * kParts + kParts + part) * blockDim.x + tid] : make_uint4(0, 0, 0, 0);
       }
     }
     float x[16];

@@ -90,8 +90,8 @@ class PagedChunk(C.Structure):
 
 
 def _kept(params, *buffers):
-    """The buffers a description names live as long as it does; its address is taken once."""
-    params._keep, params._at = buffers, C.addressof(params)
+    """The buffers a description names live as long as it does."""
+    params._keep = buffers
     return params
 
 
@@ -214,7 +214,7 @@ def _ptr(x) -> int | None:
 
 def _ref(x):
     """Address of a description structure (None: a null pointer)."""
-    return None if x is None else getattr(x, "_at", None) or C.addressof(x)
+    return None if x is None else C.addressof(x)
 
 
 def _stream(s) -> int | None:

@@ -234,7 +234,8 @@ int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *
  * sequence's positions up to its own, whatever lies in the pages behind
  * kv_lens[b]. q and out [rows][n_heads][head_dim] have the pool's type; a row
  * that sees no position gives zeros. Table entries outside [0, n_pages) read
- * page 0; kv_lens past the table count as the table's length. Any number of
+ * page 0; kv_lens past the table count as the table's length. out overlaps
+ * neither q nor the pools. Any number of
  * query heads per KV head; head_dim a multiple of 16 up to 128; scale > 0.
  * Float32 statistics and sums; results do not depend on the order in which
  * the GPU runs the parts. Scratch of a fixed size lives in `k`: the first call

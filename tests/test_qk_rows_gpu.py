@@ -80,6 +80,62 @@ def test_norm_rope(gb, kernels, cuda, ci, typ, out):
 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nk,hd,dims,halves,extra", [(5, 1, 80, 80, True, 0), (3, 2, 96, 32, False, 1),
+                                                        (12, 2, 128, 128, True, 5), (1, 1, 48, 48, False, 2),
+                                                        (40, 4, 256, 128, True, 3)])
+def test_many_rows(gb, kernels, cuda, typ, nq, nk, hd, dims, halves, extra):
+    # several rows to a CTA, the last of them with fewer; head_dims that leave lanes over
+    rows = 2664 + extra
+    g = torch.Generator().manual_seed(7)
+    qk = make(rows, nq + nk, hd, typ, 210, 2.0)
+    pos = torch.randint(0, 100000, (rows,), generator=g, dtype=torch.int32).cuda()
+    w = (1 + 0.3 * torch.randn(hd, generator=g)).cuda()
+    q_out, k_out = torch.zeros((rows, nq * hd), dtype=DT[typ], device="cuda"), torch.zeros((rows, nk * hd), dtype=DT[typ], device="cuda")
+    T, at, wide = getattr(gb, typ.upper()), qk.data_ptr(), (nq + nk) * hd
+    kernels.qk_norm_rope(T, at, wide, nq, at + nq * hd * qk.element_size(), wide, nk, rows, hd, gb.qk_norm(w, w, 1e-6),
+                         gb.rope(5e5, dims, halves), pos, T, q_out, nq * hd, k_out, nk * hd)
+    torch.cuda.synchronize()
+    y = norm(qk.double().reshape(rows, nq + nk, hd), w, 1e-6)
+    want, size = rotate(y, pos, dims, halves, 5e5), size_of(y, dims, halves)
+    close(q_out.reshape(rows, nq, hd), want[:, :nq], size[:, :nq], typ)
+    close(k_out.reshape(rows, nk, hd), want[:, nq:], size[:, nq:], typ)
+    # in place, and the same result
+    kernels.qk_norm_rope(T, at, wide, nq, at + nq * hd * qk.element_size(), wide, nk, rows, hd, gb.qk_norm(w, w, 1e-6),
+                         gb.rope(5e5, dims, halves), pos, T, at, wide, at + nq * hd * qk.element_size(), wide)
+    torch.cuda.synchronize()
+    assert torch.equal(qk, torch.cat((q_out, k_out), 1))
+
+
+@pytest.mark.parametrize("typ,pool", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+def test_append_many_rows(gb, kernels, cuda, typ, pool):
+    # more sequences than a warp looks at together, several rows to a CTA across their borders, norms on the way
+    seqs = [(37 + b % 5, 60 + b % 90) for b in range(70)] + [(0, 12), (1, 1)]
+    nq, nk, hd = 3, 2, 80
+    B = Batch(seqs, nk, hd, 16, pool, 320, first=5, pad=7)
+    qkv = make(B.rows, nq + 2 * nk, hd, typ, 420)
+    q_out = torch.full((B.rows, nq * hd), 3.0, dtype=DT[pool], device="cuda")
+    w = (1 + 0.3 * torch.randn(hd, generator=torch.Generator().manual_seed(5))).cuda()
+    kp, vp, ksize = B.k.double().clone(), B.v.double().clone(), torch.zeros(B.k.shape, dtype=torch.float64, device="cuda")
+    at, wide, e = qkv.data_ptr(), (nq + 2 * nk) * hd, qkv.element_size()
+    kernels.rope_append_paged(B.chunk(gb), getattr(gb, typ.upper()), at, wide, nq, at + nq * hd * e, wide,
+                              at + (nq + nk) * hd * e, wide, gb.rope(5e5, hd, True), q_out, nq * hd,
+                              norm=gb.qk_norm(w, w, 1e-5))
+    torch.cuda.synchronize()
+    x = qkv.double().reshape(B.rows, nq + 2 * nk, hd)
+    want, qsize = torch.full((B.rows, nq, hd), 3.0, dtype=torch.float64, device="cuda"), torch.zeros((B.rows, nq, hd), device="cuda")
+    for b, (n, kv) in enumerate(seqs):
+        r = slice(B.starts[b], B.starts[b] + n)
+        y = norm(x[r, :nq + nk], w, 1e-5)
+        z, size = rotate(y, torch.arange(kv - n, kv, device="cuda"), hd, True, 5e5), size_of(y, hd, True)
+        want[r], qsize[r] = z[:, :nq], size[:, :nq]
+        pages, slot = B.slots(b, kv - n, kv)
+        kp[pages, :, slot], vp[pages, :, slot], ksize[pages, :, slot] = z[:, nq:], x[r, nq + nk:], size[:, nq:].double()
+    close(q_out.reshape(B.rows, nq, hd), want, qsize, pool)
+    close(B.k, kp, ksize, pool)
+    assert torch.equal(B.v, vp.to(DT[pool]))
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("halves", [False, True])
 def test_in_place_and_parts(gb, kernels, cuda, typ, halves):
     # norms alone, the rotation alone, a norm of the keys alone; each output in its input's place

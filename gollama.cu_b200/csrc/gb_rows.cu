@@ -346,6 +346,7 @@ int check_rows(const char *what, const char *name, const void *p, long long ld, 
 int common(const char *what, RowArgs &a, int nq, int nk, int nv, int hd, int rows, const gb_qk_norm_params *norm,
            const gb_rope_params *rope) {
   if (rows < 0) return gb_fail(GB_ERR_INVALID, "%s: %d rows", what, rows);
+  if (rows > (1 << 30)) return gb_fail(GB_ERR_UNSUPPORTED, "%s: %d rows", what, rows);  // rows are counted in 32 bits
   if (nq < 0 || nk < 0 || nq > (1 << 16) || nk > (1 << 16))
     return gb_fail(GB_ERR_INVALID, "%s: %d query heads, %d key heads", what, nq, nk);
   if (hd < 16 || hd > kMaxHD || hd % 16)

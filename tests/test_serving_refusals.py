@@ -70,6 +70,7 @@ def test_norm_and_rotation(gb):
     r = gb.rope
     for more, code, word in (
             (dict(typ=2), 3, "types 2"), (dict(out=14), 3, "types"), (dict(rows=-1), 1, "-1 rows"),
+            (dict(rows=(1 << 30) + 1), 3, "rows"),
             (dict(heads=-1), 1, "query heads"), (dict(hd=24), 3, "head_dim 24"), (dict(hd=272), 3, "head_dim 272"),
             (dict(q=None), 1, "q is null"), (dict(q_out=None), 1, "q_out is null"), (dict(k=None), 1, "k is null"),
             (dict(k_out=4104), 1, "16-byte"), (dict(ldq=500), 1, "apart"), (dict(ldk=120), 1, "apart"),
@@ -124,7 +125,8 @@ def line_pieces(seqs, G, n_kv, RU, KT, grid, wide, narrow, opening, cap=1 << 30)
 
 
 @pytest.mark.parametrize("RU,KT,grid,costs", [(64, 64, 296, (1, 1, 0)), (256, 128, 148, (4, 2, 2)), (64, 64, 3, (1, 1, 0)),
-                                              (256, 128, 7, (4, 2, 2))])
+                                              (256, 128, 7, (4, 2, 2)), (256, 128, 148, (4, 2, 4)),
+                                              (128, 64, 296, (1, 1, 0)), (64, 32, 296, (1, 1, 0))])
 def test_every_tile_has_one_cta_and_every_unit_its_joiners(RU, KT, grid, costs):
     import random
     r = random.Random(RU + grid)

@@ -13,8 +13,8 @@
 // Split of the work: the (unit, tile) pairs of all sequences form one line,
 // cut into equal runs, one for each CTA of a grid that fills the GPU once. A
 // unit cut by a run's end leaves its partial rows (maximum, sum, unnormalised
-// output) in the workspace; the last CTA to arrive at that unit joins them in
-// CTA order, so the result does not depend on which one that is. One rule
+// output) in the workspace, where they are joined in CTA order once all are
+// there, so the result does not depend on which CTA does it. One rule
 // serves one sequence decoding (a line of few units cut 148 ways), long
 // prompts (whole units, cut only at the ends) and mixtures of both.
 #include <math.h>
@@ -53,7 +53,7 @@ struct Seq {
 };
 GB_DEV Seq seq_of(const ChunkArgs &a, int b) {
   Seq s;
-  const int lo = max(0, a.c.q_start[b]), hi = min(a.c.rows, a.c.q_start[b + 1]);
+  const int lo = max(0, a.c.q_start[b]), hi = min(a.c.rows, max(lo, a.c.q_start[b + 1]));
   const int len = a.c.kv_lens[b];
   s.q0 = lo;
   s.n = max(0, hi - lo);
@@ -769,11 +769,12 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
 //
 // K and V tiles come in order K0 V0 K1 V1 ... into a ring, with the 128-byte
 // swizzle that the descriptors name. Where the page size has a divisor of at
-// least 8 in common with the tile, two warps fetch them by TMA, a box of that
-// many rows to a lane, from wherever its page lies; what a box brings behind
-// the sequence's end is overwritten with zeros in V (0 NaN is NaN), and does
-// not matter in K. Other page sizes go through 16-byte asynchronous copies by
-// three warps, zeros behind the end. One thread issues all tcgen05.mma; they
+// least 8 in common with the tile, one warp fetches K and one V by TMA, in boxes
+// of that many rows from wherever their page lies; what a box brings behind
+// the sequence's end is overwritten with zeros in V (0 NaN is NaN) by a third
+// warp, which also brings the queries, and does not matter in K. Other page
+// sizes go through 16-byte asynchronous copies by the three warps, zeros behind
+// the end. One thread issues all tcgen05.mma; they
 // run in the order issued, so S of the next tile may be queued behind the P V
 // that reads P in the same columns.
 //
@@ -795,7 +796,7 @@ constexpr uint32_t kChunkBytes = 128 * 128;  // 128 rows of 64 elements
 constexpr int kRingBytes = 10 * kChunkBytes;
 template <int HD>
 constexpr int ring_slots() { return kRingBytes / (HD / 64 * (int)kChunkBytes); }
-constexpr int kHeader = 3072;  // tiles lie on 1024-byte boundaries behind it
+constexpr int kHeader = 3 * 1024;  // tiles lie on 1024-byte boundaries behind it
 template <int HD>
 constexpr int tc_smem() { return kHeader + 2 * HD / 64 * (int)kChunkBytes + kRingBytes; }
 
@@ -890,13 +891,15 @@ GB_DEV uint32_t idesc_of(int N, bool TB) {
 
 // Every wait is bounded: when one runs out, or another thread's has, the CTA
 // goes on without waiting (all addresses stay within their buffers), ends, and
-// the error word tells.
+// the error word tells. `tiles`: how many tiles' work the wait spans, of any
+// length in a long sequence.
 // The CTA's last waits (`last`: for copies and products in flight) are made all the same.
-GB_DEV void bar_wait(TcShared *sh, uint64_t *bar, uint32_t parity, unsigned *err, bool last = false) {
-  for (uint32_t i = 0; i < GB_WAIT_LIMIT; i++) {
-    if (gb_mbar_try_wait(bar, parity)) return;
-    if (!last && (i & 63) == 63 && *(volatile int *)&sh->dead) return;
-  }
+GB_DEV void bar_wait(TcShared *sh, uint64_t *bar, uint32_t parity, unsigned *err, bool last = false, int tiles = 1) {
+  for (int t = 0; t < tiles; t++)
+    for (uint32_t i = 0; i < GB_WAIT_LIMIT; i++) {
+      if (gb_mbar_try_wait(bar, parity)) return;
+      if (!last && (i & 63) == 63 && *(volatile int *)&sh->dead) return;
+    }
   *(volatile int *)&sh->dead = 1;
   *(volatile unsigned *)err = GB_DEVERR_TIMEOUT;
 }
@@ -1114,15 +1117,17 @@ __global__ void __launch_bounds__(kTN, 1)
     // ---- queries, and zeros over V behind the sequence's end
     const int ppr = hd / 8;
     uint32_t n0 = 0, pieces = 0, phase = 0;  // bit i: parity of the next landing in slot i
+    int before = 1;                          // tiles of the piece before
     while (w.next(a)) {
-      bar_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err);
+      bar_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err, false, before);
+      before = w.t1 - w.t0;
       load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, 0, 1, ppr, lane);
       cp_async_arrive(&sh->q_full);
       pieces++;
       const int last = w.s.cap / kTT;  // the tile that the end lies in
       if (last >= w.t0 && last < w.t1) {
         const uint32_t slot = (n0 + 2 * (last - w.t0) + 1) % NS;
-        bar_wait(sh, &sh->landed[slot], phase >> slot & 1, a.err);
+        bar_wait(sh, &sh->landed[slot], phase >> slot & 1, a.err, false, before);
         phase ^= 1u << slot;
         for (int i = (w.s.cap % kTT) * 8 + lane; i < kTT * 8; i += 32)
           for (int c = 0; c < HD / 64; c++)

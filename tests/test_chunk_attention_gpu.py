@@ -329,3 +329,40 @@ def test_an_infinite_key_shows(gb, kernels, cuda, typ):
     call(gb, kernels, B, q, 4, 0.125, out)
     torch.cuda.synchronize()
     assert out[:30].isnan().all() and out[30:].isfinite().all()
+
+
+def test_a_falling_q_start_has_no_rows(gb, kernels, cuda):
+    # the difference of two of its entries may pass 32 bits
+    B = Batch([(2, 48), (1, 9)], 2, 64, 16, "f16", 190)
+    q = torch.randn((3, 4 * 64), generator=torch.Generator().manual_seed(7)).half().cuda()
+    for starts in ([1, -2 ** 31, 0], [2 ** 31 - 1, -2 ** 31, -2 ** 31], [2 ** 31 - 1, 2 ** 31 - 1, 0]):
+        B.q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        out = torch.full_like(q, 5)
+        call(gb, kernels, B, q, 4, 0.125, out)
+        torch.cuda.synchronize()
+        assert (out == 5).all(), starts
+
+
+def test_a_unit_of_many_tiles(gb, cuda):
+    # 2^22 positions, all of them the slots of one page: a unit of 256 rows takes 32768 tiles, and no wait that
+    # spans them runs out (the next call would say so). Scores are zero and values one: sums of ones below 2^24
+    # are exact, and their quotient is off by the reciprocal's and the product's half steps, which the result's
+    # type rounds away.
+    k = gb.Kernels(0)
+    try:
+        n, kv, page = 512, 1 << 22, 128
+        pool = torch.zeros((2, 1, 1, page, 64), dtype=torch.float16, device="cuda")
+        pool[1] = 1
+        table = torch.zeros((1, kv // page), dtype=torch.int32, device="cuda")
+        starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        lens = torch.tensor([kv], dtype=torch.int32, device="cuda")
+        c = gb.paged_chunk(n, 1, starts, lens, table, kv // page, 1, page, 1, 64, gb.F16, pool[0], pool[1])
+        heads = 148 * 256 // n  # enough rows for a whole unit or more to each CTA
+        q = torch.ones((n, heads * 64), dtype=torch.float16, device="cuda")
+        out = torch.zeros_like(q)
+        for _ in range(2):
+            k.attn_chunk_paged(c, q, heads * 64, heads, 0.125, out, heads * 64)
+            torch.cuda.synchronize()
+        assert (out == 1).all()
+    finally:
+        k.close()

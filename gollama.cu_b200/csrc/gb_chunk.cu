@@ -801,7 +801,7 @@ template <int HD>
 constexpr int tc_smem() { return kHeader + 2 * HD / 64 * (int)kChunkBytes + kRingBytes; }
 
 struct TcShared {
-  uint64_t full[10], empty[10], landed[10], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free, fin;
+  uint64_t full[10], empty[10], landed[10], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_free, fin;
   PlanShared plan;
   Plan mine;  // this CTA's, for its end
   uint32_t tmem;
@@ -999,7 +999,7 @@ GB_DEV uint64_t add2(uint64_t x, uint64_t y) {
 // for a tile outgrows the schedulers' instruction caches, and fetching it took as
 // long as running it (stalls on no instruction as many as issues).
 template <int T, bool BOTH>
-GB_DEV float weights(uint32_t s_at, int rel, bool cut, float scale, float shift) {
+GB_DEV float weights(uint32_t s_at, int rel, bool cut, float scale, float shift, uint64_t *full) {
   const uint64_t k2 = pair(scale, scale), c2 = pair(shift, shift);
   uint64_t sum[2] = {0, 0};
 #pragma unroll 1
@@ -1020,6 +1020,10 @@ GB_DEV float weights(uint32_t s_at, int rel, bool cut, float scale, float shift)
     }
     tc_st16(s_at + 32 * h, u);
     if (!BOTH) tc_st16(s_at + 32 * h + 16, rest);
+    tc_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) gb_mbar_arrive(full + h);
   }
   float x, y;
   unpair(add2(sum[0], sum[1]), x, y);
@@ -1045,7 +1049,8 @@ __global__ void __launch_bounds__(kTN, 1)
     } else if (lane < NS + 2) {
       const int g = lane - NS;
       gb_mbar_init(&sh->s_full[g], 1);
-      gb_mbar_init(&sh->p_full[g], kSoftWarps / 2);
+      gb_mbar_init(&sh->p_full[g][0], kSoftWarps / 2);
+      gb_mbar_init(&sh->p_full[g][1], kSoftWarps / 2);
       gb_mbar_init(&sh->pv_done[g], 1);
     } else if (lane == 31) {
       gb_mbar_init(&sh->q_full, (TMA ? 1 : kLoadWarps) * 32);
@@ -1195,17 +1200,25 @@ __global__ void __launch_bounds__(kTN, 1)
     };
     // O_g (+)= P_g V, V at ring position n
     auto pv = [&](int g, uint32_t n, bool first, bool both, bool v_done) {
-      const uint32_t v_at = ring + n % NS * kTile;
+      const uint32_t v_at = ring + n % NS * kTile, parity = (g ? np1++ : np0++) & 1;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        bar_wait(sh, &sh->p_full[g][h], parity, a.err);
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < kTT / 32; k++) {
+            const int kk = 4 * (k >> 1) + 2 * h + (k & 1);
+            tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + p_column(kk), desc_rows(v_at + kk * 2048, kChunkBytes), iv,
+                      !first || h || k);
+            if (!both)
+              tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + p_column(kk) + 16,
+                        desc_rows(v_at + kk * 2048, kChunkBytes), iv, 1);
+          }
+        }
+        __syncwarp();
+      }
       if (leader) {
-#pragma unroll
-        for (int kk = 0; kk < kTT / 16; kk++)
-          tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + p_column(kk), desc_rows(v_at + kk * 2048, kChunkBytes), iv,
-                    !first || kk != 0);
-        if (!both)
-#pragma unroll
-          for (int kk = 0; kk < kTT / 16; kk++)
-            tc_mma_ta(tmem + 256 + g * 128, tmem + g * 128 + p_column(kk) + 16, desc_rows(v_at + kk * 2048, kChunkBytes),
-                      iv, 1);
         tc_commit(&sh->pv_done[g]);
         if (v_done) tc_commit(&sh->empty[n % NS]);
       }
@@ -1215,10 +1228,6 @@ __global__ void __launch_bounds__(kTN, 1)
       bar_wait(sh, &sh->full[n % NS], n / NS & 1, a.err);
       // the asynchronous copies' bytes, seen here, before the tensor cores read them (about 400 cycles)
       if (!TMA) gb_fence_proxy_async();
-    };
-    auto p_ready = [&](int g) {
-      bar_wait(sh, &sh->p_full[g], (g ? np1++ : np0++) & 1, a.err);
-      tc_fence_after();
     };
     while (w.next(a)) {
       const int n = w.t1 - w.t0;
@@ -1242,15 +1251,12 @@ __global__ void __launch_bounds__(kTN, 1)
         loaded(v);
         if (both) {
           if (t + 1 < n) loaded(v + 1);
-          p_ready(0);
           pv(0, v, t == 0, true, false);
           if (t + 1 < n) qk(0, 0, v + 1, false, false);
-          p_ready(1);
           pv(1, v, t == 0, true, true);
           if (t + 1 < n) qk(1, 1, v + 1, true, t + 2 == n);
         } else {
           const int g = t & 1;
-          p_ready(g);
           pv(g, v, t < 2, false, true);
           if (t + 2 < n) {
             loaded(v + 3);
@@ -1329,13 +1335,11 @@ __global__ void __launch_bounds__(kTN, 1)
           }
           m = mn;
           const float ms = m == -INFINITY ? 0.f : m;
-          l += both ? weights<T, true>(s_at, rel, cut, a.scale_log2, -ms)
-                    : weights<T, false>(s_at, rel, cut, a.scale_log2, -ms);
-          tc_wait_st();
+          l += both ? weights<T, true>(s_at, rel, cut, a.scale_log2, -ms, sh->p_full[g])
+                    : weights<T, false>(s_at, rel, cut, a.scale_log2, -ms, sh->p_full[g]);
+        } else if (lane < 2) {
+          gb_mbar_arrive(&sh->p_full[g][lane]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) gb_mbar_arrive(&sh->p_full[g]);
       }
       // ---- the unit's end: its rows out of tensor memory. The threads of a row
       // (two, or four where both groups have it) tell each other their sums,

@@ -36,6 +36,7 @@ struct ChunkArgs {
   void *out;
   long long ldq, ldo;
   int n_heads, G;
+  int q_tokens;       // of a TMA box of queries (0: none)
   float scale_log2;   // scale * log2(e): the softmax is taken in powers of two
   float *part;        // partial rows (part_slot)
   unsigned *counter;  // [CTAs][kCounters], zero between launches
@@ -85,9 +86,9 @@ struct Line {
   static GB_DEV long long seq_cost(const ChunkArgs &a, const Seq &s) {
     const int lane = threadIdx.x & 31, nu = units(s, a.G);
     long long t = 0;
-    if (nu <= 16)
+    if (nu <= 4)
       for (int u = 0; u < nu; u++) t += cost(s, a.G, u);
-    for (unsigned many = __ballot_sync(0xffffffffu, nu > 16); many; many &= many - 1) {
+    for (unsigned many = __ballot_sync(0xffffffffu, nu > 4); many; many &= many - 1) {
       const int from = __ffs(many) - 1;
       Seq o;
       o.q0 = 0, o.n = __shfl_sync(0xffffffffu, s.n, from), o.len0 = __shfl_sync(0xffffffffu, s.len0, from);
@@ -963,6 +964,14 @@ GB_DEV void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t
       : "memory");
 }
 
+GB_DEV void tma_box3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(gb_smem_u32(bar))
+      : "memory");
+}
+
 // What a packed pair leaves of (x, y): the remainder, exact in float32.
 template <int T>
 GB_DEV uint32_t pack2_rest(float x, float y, uint32_t p) {
@@ -1033,7 +1042,7 @@ GB_DEV float weights(uint32_t s_at, int rel, bool cut, float scale, float shift,
 template <int T, int HD, bool TMA>
 __global__ void __launch_bounds__(kTN, 1)
     attn_chunk_tc_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap k_map,
-                         const __grid_constant__ CUtensorMap v_map) {
+                         const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map) {
   extern __shared__ __align__(1024) uint8_t tc_raw[];
   TcShared *const sh = (TcShared *)tc_raw;
   const uint32_t q_at = gb_smem_u32(tc_raw) + kHeader;
@@ -1067,9 +1076,10 @@ __global__ void __launch_bounds__(kTN, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // a wide tile takes 4,000 clocks, a narrow one 2,200, what a piece has before and behind its tiles some 2,000
-  const Plan plan = make_plan<kTR, kTT, 4, 2, 4, kTN>(a, &sh->plan);
-  Walk<kTR, kTT, 4, 2, 4> w;
+  // A wide tile takes 4,000 clocks, a narrow one 2,200, and what a piece has before and behind its tiles some 6,000
+  // (counted as 4,000, 12 ragged sequences took 111 us instead of 105; as twice a tile of the unit's kind, 112)
+  const Plan plan = make_plan<kTR, kTT, 4, 2, 6, kTN>(a, &sh->plan);
+  Walk<kTR, kTT, 4, 2, 6> w;
   w.start(a, plan);
   if (tid == 0) sh->mine = plan;
   tc_fence_before();
@@ -1121,13 +1131,30 @@ __global__ void __launch_bounds__(kTN, 1)
   } else if (TMA && warp == kSoftWarps + 2) {
     // ---- queries, and zeros over V behind the sequence's end
     const int ppr = hd / 8;
+    const uint32_t leader = elect_lane();
     uint32_t n0 = 0, pieces = 0, phase = 0;  // bit i: parity of the next landing in slot i
     int before = 1;                          // tiles of the piece before
     while (w.next(a)) {
       bar_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err, false, before);
       before = w.t1 - w.t0;
-      load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, 0, 1, ppr, lane);
-      cp_async_arrive(&sh->q_full);
+      // Where 128 packed rows are whole tokens' heads they are a box: 256 rows took this warp 4.4 us by
+      // copies of its own. The box brings rows past the unit's too, which nobody looks at; few rows are copied.
+      // (After a wait that ran out none is asked for: one at most is ever on its way.)
+      if (a.q_tokens && w.nr > 32 && !__any_sync(0xffffffffu, *(volatile int *)&sh->dead)) {
+        const int halves = w.nr > 128 ? 2 : 1;
+        if (lane == 0) gb_mbar_expect_tx(&sh->q_full, halves * kTile);
+        else gb_mbar_arrive(&sh->q_full);
+        __syncwarp();
+        if (leader)
+          for (int i = 0; i < halves; i++)
+            for (int c = 0; c < HD / 64; c++)
+              tma_box3(q_at + i * kTile + c * kChunkBytes, &q_map, 64 * c, w.head * a.G,
+                       w.s.q0 + w.r0 / a.G + i * a.q_tokens, &sh->q_full);
+        __syncwarp();
+      } else {
+        load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, 0, 1, ppr, lane);
+        cp_async_arrive(&sh->q_full);
+      }
       pieces++;
       const int last = w.s.cap / kTT;  // the tile that the end lies in
       if (last >= w.t0 && last < w.t1) {
@@ -1146,6 +1173,7 @@ __global__ void __launch_bounds__(kTN, 1)
       n0 += 2 * (w.t1 - w.t0);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (pieces) bar_wait(sh, &sh->q_full, (pieces - 1) & 1, a.err, true);
   } else if (!TMA && warp >= kSoftWarps && warp < kMmaWarp) {
     // ---- queries, K and V by asynchronous copies
     // A tile's four blocks of 32 rows go round the three warps, one block on with each tile.
@@ -1489,9 +1517,9 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// A pool as rows of head_dim 16-bit elements, in boxes of 64 columns by `br`
-// rows (zeros past head_dim).
-int pool_map(const ChunkArgs &a, void *pool, int br, CUtensorMap *map, const char *what) {
+// 16-bit elements in boxes whose rows are 64 of them, zeros past the dims.
+int tensor_map(void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+               CUtensorMap *map, const char *what) {
   static EncodeTiledFn encode = nullptr;
   if (!encode) {
     void *fn = nullptr;
@@ -1501,29 +1529,46 @@ int pool_map(const ChunkArgs &a, void *pool, int br, CUtensorMap *map, const cha
       return gb_fail(GB_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
     encode = (EncodeTiledFn)fn;
   }
-  const cuuint64_t dims[2] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.c.n_pages * a.c.n_kv * a.c.page_size};
-  const cuuint64_t strides[1] = {(cuuint64_t)a.c.head_dim * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)br}, one[2] = {1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, pool, dims, strides, box, one,
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, base, dims, strides, box, one,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return gb_fail(GB_ERR_CUDA, "%s: tensor map encode failed (%d)", what, (int)r);
   return GB_OK;
 }
 
+// A pool as rows of head_dim elements, in boxes of `br` rows.
+int pool_map(const ChunkArgs &a, void *pool, int br, CUtensorMap *map, const char *what) {
+  const cuuint64_t dims[2] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.c.n_pages * a.c.n_kv * a.c.page_size};
+  const cuuint64_t strides[1] = {(cuuint64_t)a.c.head_dim * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)br};
+  return tensor_map(pool, 2, dims, strides, box, map, what);
+}
+
+// The queries [rows][n_heads][head_dim], in boxes of a KV head's G heads of 128 / G tokens.
+int query_map(const ChunkArgs &a, CUtensorMap *map, const char *what) {
+  const cuuint64_t dims[3] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.c.rows};
+  const cuuint64_t row = a.c.rows > 1 ? (cuuint64_t)a.ldq : (cuuint64_t)a.n_heads * a.c.head_dim;  // of one row: any
+  const cuuint64_t strides[2] = {(cuuint64_t)a.c.head_dim * 2, row * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)a.q_tokens};
+  return tensor_map((void *)a.q, 3, dims, strides, box, map, what);
+}
+
 template <int T, int HD, bool TMA>
-int launch_tc(const ChunkArgs &a, int sms, cudaStream_t st, const char *what) {
-  CUtensorMap k_map = {}, v_map = {};
+int launch_tc(ChunkArgs a, int sms, cudaStream_t st, const char *what) {
+  CUtensorMap k_map = {}, v_map = {}, q_map = {};
   if (TMA) {
     const int br = box_rows(a.c.page_size);
     int rc = pool_map(a, a.c.k_pool, br, &k_map, what);
     if (rc == GB_OK) rc = pool_map(a, a.c.v_pool, br, &v_map, what);
+    a.q_tokens = 128 % a.G ? 0 : 128 / a.G;
+    if (rc == GB_OK && a.q_tokens) rc = query_map(a, &q_map, what);
     if (rc != GB_OK) return rc;
   }
   GB_CUDA(cudaFuncSetAttribute(attn_chunk_tc_kernel<T, HD, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                tc_smem<HD>()),
           what);
-  attn_chunk_tc_kernel<T, HD, TMA><<<(unsigned)sms, kTN, tc_smem<HD>(), st>>>(a, k_map, v_map);
+  attn_chunk_tc_kernel<T, HD, TMA><<<(unsigned)sms, kTN, tc_smem<HD>(), st>>>(a, k_map, v_map, q_map);
   GB_CUDA(cudaGetLastError(), what);
   return GB_OK;
 }

@@ -366,3 +366,18 @@ def test_a_unit_of_many_tiles(gb, cuda):
         assert (out == 1).all()
     finally:
         k.close()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,n", [(8, 9), (8, 40), (3, 30), (1, 140)])
+def test_nan_queries_stay_in_their_rows(gb, kernels, cuda, typ, heads, n):
+    # the rows behind a sequence's are another's (or nobody's), whatever they hold
+    B = Batch([(n, 300), (7, 90), (n, n)], 1, 64, 16, typ, 200, pad=3)
+    q = torch.randn((B.rows, heads * 64), generator=torch.Generator().manual_seed(8)).to(DT[typ]).cuda()
+    out = torch.full_like(q, 7)
+    want, mag, big = B.attention(q, heads, 0.125, out)
+    q[n:n + 7], q[2 * n + 7:] = float("nan"), float("inf")
+    call(gb, kernels, B, q, heads, 0.125, out)
+    torch.cuda.synchronize()
+    fine = ((out.double() - want).abs() <= bound(typ, 64, 300, want, mag, big)).all(1)
+    assert fine[:n].all() and fine[n + 7:].all() and out[n:n + 7].isnan().all()

@@ -125,7 +125,7 @@ def line_pieces(seqs, G, n_kv, RU, KT, grid, wide, narrow, opening, cap=1 << 30)
 
 
 @pytest.mark.parametrize("RU,KT,grid,costs", [(64, 64, 296, (1, 1, 0)), (256, 128, 148, (4, 2, 2)), (64, 64, 3, (1, 1, 0)),
-                                              (256, 128, 7, (4, 2, 2)), (256, 128, 148, (4, 2, 4)),
+                                              (256, 128, 7, (4, 2, 2)), (256, 128, 148, (4, 2, 6)),
                                               (128, 64, 296, (1, 1, 0)), (64, 32, 296, (1, 1, 0))])
 def test_every_tile_has_one_cta_and_every_unit_its_joiners(RU, KT, grid, costs):
     import random

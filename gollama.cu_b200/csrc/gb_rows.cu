@@ -23,7 +23,7 @@
 namespace {
 
 constexpr int kMaxHD = 256;       // head_dim
-constexpr int kMaxThreads = 320;  // threads of a CTA, a task each
+constexpr int kMaxThreads = 192;  // threads of a CTA, a task each
 
 struct RowArgs {
   const void *q, *k, *v;  // rows of n_heads / n_kv / n_kv heads (v only for the append)
@@ -131,9 +131,7 @@ GB_DEV const void *task_source(const RowArgs &a, const Task &k, long long *at, l
 // Waits until at most n of this thread's groups of copies (n known when the loop
 // over rows is unrolled) are on their way.
 GB_DEV void rows_landed(int n) {
-  if (n >= 5) asm volatile("cp.async.wait_group 5;" ::: "memory");
-  else if (n == 4) asm volatile("cp.async.wait_group 4;" ::: "memory");
-  else if (n == 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  if (n >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
   else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
   else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
   else asm volatile("cp.async.wait_all;" ::: "memory");
@@ -142,18 +140,19 @@ GB_DEV void rows_landed(int n) {
 // R rows by a slice of their heads to a CTA, a thread to the same 16 elements of
 // a head in each row: all rows' elements are on their way while the rows'
 // sequences are looked up (by each warp for itself) and their R dims/2 angles
-// formed, once for all heads. With few rows R is 1, for the most CTAs. With many
-// it is 6 (3 in float32), the elements on their way to shared memory, where a
-// thread reads what it asked for: 8192 rows of 72 heads of 128 took 84 us with
-// one row to a CTA, and as long with four held in registers, of which an SM has
-// too few to keep the memory busy; this way 61 us, 5.0 TB/s of what it reads and
-// writes. Few rows are bound by the launch: 2.3 us for one, 3 for 64 with their
-// append (launches of one graph).
+// formed, once for all heads. R is 1, or 4 for norms of 2^26 elements and more in 16 bits,
+// the elements then on their way to shared memory, where a thread reads what it
+// asked for. 8192 rows of 72 heads of 128 take 59 us so, 5.1 TB/s of what they
+// read and write, and 64 with a CTA to a row; of 40 heads 36 either way; with
+// float32 rows, of which two fit, 60 against 43, and the append of 8192 rows of
+// 48 heads 33.5 against 31. CTAs of up to 192 threads: 320 took 66, 37, 47 and
+// 31, 128 took 64, 40, 46 and 30.5. Few rows are bound by the launch: 2.3 us for
+// one, 3 for 64 with their append (launches of one graph).
 template <int TI, int TO, bool APPEND, int R>
-__global__ void __launch_bounds__(kMaxThreads, R > 1 ? 3 : 1) head_rows_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kParts = sizeof(Raw<TI>) / 16;  // 16-byte parts of eight elements
+__global__ void __launch_bounds__(kMaxThreads, R > 1 ? 5 : 1) head_rows_kernel(const __grid_constant__ RowArgs a) {
+  static_assert(R == 1 || (sizeof(Raw<TI>) == 16 && !APPEND), "rows by way of shared memory");
   __shared__ float2 cs[R][kMaxHD / 2];          // pair j of row i at [i][(j % 8) * half / 8 + j / 8]
-  extern __shared__ uint4 stage[];              // [row][part of both runs][thread]
+  extern __shared__ uint4 stage[];              // [row][run][thread]
   const int row0 = blockIdx.x * R, tid = threadIdx.x, lane = tid & 31, half = a.dims / 2, eighth = half / 8;
   const Task k = task_of(a, (int)(blockIdx.y * blockDim.x) + tid);
   Raw<TI> xa = {}, xb = {};
@@ -166,19 +165,15 @@ __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 3 : 1) head_rows_kernel(c
     }
   } else {
     const uint32_t to = gb_smem_u32(stage + tid);
-    constexpr int kSize = TI == GB_F32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < R; i++) {
       if (k.on && row0 + i < a.rows) {
-        const uint8_t *from = (const uint8_t *)src + ((row0 + i) * ld + src_at) * kSize;
+        const uint16_t *from = (const uint16_t *)src + (row0 + i) * ld + src_at;
 #pragma unroll
-        for (int part = 0; part < 2 * kParts; part++) {
-          const uint8_t *at = from + (part < kParts ? k.dA * kSize + part * 16 : k.dB * kSize + (part - kParts) * 16);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                           to + (uint32_t)(i * 2 * kParts + part) * blockDim.x * 16),
-                       "l"(at)
+        for (int run = 0; run < 2; run++)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (uint32_t)(2 * i + run) * blockDim.x * 16),
+                       "l"(from + (run ? k.dB : k.dA))
                        : "memory");
-        }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
@@ -232,12 +227,9 @@ __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 3 : 1) head_rows_kernel(c
   for (int i = 0; i < R; i++) {
     if constexpr (R > 1) {
       rows_landed(R - 1 - i);
-#pragma unroll
-      for (int part = 0; part < kParts; part++) {
-        // lanes past head_dim asked for nothing and add nothing to their head's sum
-        xa.u[part] = k.on ? stage[(i * 2 * kParts + part) * blockDim.x + tid] : make_uint4(0, 0, 0, 0);
-        xb.u[part] = k.on ? stage[(i * 2 * kParts + kParts + part) * blockDim.x + tid] : make_uint4(0, 0, 0, 0);
-      }
+      // lanes past head_dim asked for nothing and add nothing to their head's sum
+      xa.u[0] = k.on ? stage[2 * i * blockDim.x + tid] : make_uint4(0, 0, 0, 0);
+      xb.u[0] = k.on ? stage[(2 * i + 1) * blockDim.x + tid] : make_uint4(0, 0, 0, 0);
     }
     float x[16];
     values8<TI>(xa, x);
@@ -302,15 +294,18 @@ int launch_types(const RowArgs &a, cudaStream_t st, const char *what) {
   // a task to a thread: slices of the heads beside one another
   const int tasks = (a.nq + a.nk + a.nv) << a.lph_log2, slices = (tasks + kMaxThreads - 1) / kMaxThreads;
   const int threads = ((tasks + slices - 1) / slices + 31) / 32 * 32;
-  // several rows to a CTA once that leaves every SM its three CTAs
-  constexpr int R = I == GB_F32 ? 3 : 6;
-  if (a.rows >= 148 * 3 * R) {
-    const int smem = R * threads * 2 * (int)sizeof(Raw<I>);
-    GB_CUDA(cudaFuncSetAttribute(head_rows_kernel<I, O, APPEND, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
-    head_rows_kernel<I, O, APPEND, R><<<dim3((unsigned)((a.rows + R - 1) / R), (unsigned)slices), (unsigned)threads, smem, st>>>(a);
-  } else {
-    head_rows_kernel<I, O, APPEND, 1><<<dim3((unsigned)a.rows, (unsigned)slices), (unsigned)threads, 0, st>>>(a);
+  if constexpr (!APPEND && I != GB_F32) {
+    constexpr int R = 4;
+    if ((long long)a.rows * (a.nq + a.nk) * a.hd >= 1 << 26) {
+      const int smem = R * threads * 2 * (int)sizeof(Raw<I>);
+      GB_CUDA(cudaFuncSetAttribute(head_rows_kernel<I, O, APPEND, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
+      head_rows_kernel<I, O, APPEND, R>
+          <<<dim3((unsigned)((a.rows + R - 1) / R), (unsigned)slices), (unsigned)threads, smem, st>>>(a);
+      GB_CUDA(cudaGetLastError(), what);
+      return GB_OK;
+    }
   }
+  head_rows_kernel<I, O, APPEND, 1><<<dim3((unsigned)a.rows, (unsigned)slices), (unsigned)threads, 0, st>>>(a);
   GB_CUDA(cudaGetLastError(), what);
   return GB_OK;
 }

@@ -84,8 +84,8 @@ def test_norm_rope(gb, kernels, cuda, ci, typ, out):
                                                         (12, 2, 128, 128, True, 5), (1, 1, 48, 48, False, 2),
                                                         (40, 4, 256, 128, True, 3)])
 def test_many_rows(gb, kernels, cuda, typ, nq, nk, hd, dims, halves, extra):
-    # several rows to a CTA, the last of them with fewer; head_dims that leave lanes over
-    rows = 2664 + extra
+    # several rows to a CTA (from 2^26 elements on), the last of them with fewer; head_dims that leave lanes over
+    rows = -(-(1 << 26) // (4 * (nq + nk) * hd)) * 4 + extra
     g = torch.Generator().manual_seed(7)
     qk = make(rows, nq + nk, hd, typ, 210, 2.0)
     pos = torch.randint(0, 100000, (rows,), generator=g, dtype=torch.int32).cuda()

@@ -783,14 +783,21 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
 // that reads P in the same columns.
 //
 // The running maximum is let lag: the sums and outputs are rescaled only when
-// a tile's maximum exceeds it by more than 2^kSlack, so P stays below 2^8
-// (binary16 holds 65504) and most tiles leave O in tensor memory alone.
+// a tile's maximum exceeds it by more than 2^kSlack, so most tiles leave O in
+// tensor memory alone. In binary16, whose numbers end at 2^-24, the reference
+// that a row's powers are taken from lies 2^kLift below the maximum (the sums
+// and outputs have the same factor, and their quotient has none): P stays below
+// 2^15 of the 65504 that the type holds, and a weight vanishes below 2^-32 of
+// the row's largest, not below 2^-25, where many positions beside one that
+// outweighs them would have lost up to 2^-25 each, all to the same side. A
+// position adds 2^-32 at most to the error so.
 //
 // The tensor cores take P in 16 bits. A unit of more than 128 rows rounds it
 // to the pool's type, as its result is rounded. Smaller units, which the
 // cache's bytes bound, have room for P in two parts, the rounded one and the
 // rounding's remainder (two products with V, in S's columns), and so none of
-// that error: few rows over few outstanding positions do not average it out.
+// that error but the numbers' end: few rows over few outstanding positions do
+// not average it out.
 //
 // Measured in one graph: 64 sequences decoding at 1,200 to 8,000 positions (32
 // heads over 8, head_dim 128) 208 us, 5.8 TB/s of the cache's bytes; 2048 rows of
@@ -802,6 +809,8 @@ constexpr int kTR = 256, kTT = 128;       // rows of a unit, positions of a tile
 constexpr int kSoftWarps = 16, kLoadWarps = 3, kMmaWarp = kSoftWarps + kLoadWarps;
 constexpr int kTN = (kMmaWarp + 1) * 32;  // threads
 constexpr float kSlack = 8.f;
+template <int T>
+constexpr float kLift = T == GB_F16 ? 7.f : 0.f;
 constexpr int kSlice = 64, kPolls = 64;  // rows joined at a time; polls (some 0.8 us) for a unit's other holders
 constexpr uint32_t kChunkBytes = 128 * 128;  // 128 rows of 64 elements
 constexpr int kRingBytes = 10 * kChunkBytes;
@@ -1353,8 +1362,8 @@ __global__ void __launch_bounds__(kTN, 1)
           *my_top = top;
           pair_sync();
           top = fmaxf(top, *other_top) * a.scale_log2;
-          const bool raise = top > m + kSlack || m == -INFINITY;
-          const float mn = raise ? fmaxf(m, top) : m;
+          const bool raise = top > m + (kSlack + kLift<T>) || m == -INFINITY;
+          const float mn = raise ? fmaxf(m, top - kLift<T>) : m;
           if (__any_sync(0xffffffffu, raise)) {
             const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
             l *= f;

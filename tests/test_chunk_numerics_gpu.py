@@ -1,0 +1,49 @@
+"""Attention of new rows over the pages where its numbers are at their limits:
+weights far below a row's largest, NaN and infinities that the rows see, units
+of one kind and the other, calls of fewer rows than their sequences bring."""
+import pytest
+import torch
+
+from serving_ref import DT, Batch
+from test_chunk_attention_gpu import bound, call
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["f32", "f16", "bf16"]
+
+
+def place(B, b, lo, hi, k=None, v=None):
+    """Keys and values of positions [lo, hi) of sequence b: scalars, or one number for each position."""
+    pages, slot = B.slots(b, lo, hi)
+    for pool, x in ((B.k, k), (B.v, v)):
+        if x is not None:
+            x = torch.as_tensor(x, dtype=torch.float64, device="cuda")
+            pool[pages, :, slot] = (x[:, None, None] if x.dim() else x).to(pool.dtype)
+
+
+def queries(B, heads, value=1.0):
+    return torch.full((B.rows, heads * B.hd), value, dtype=DT[B.typ], device="cuda")
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n", [1, 70])  # units of few rows, whose weights have two parts, and of more than 128
+def test_many_small_weights_beside_a_large_one(gb, kernels, cuda, typ, n):
+    # Position 0 outweighs each of the others by 17 to 20 in the exponent and its value is 0, so the result is what
+    # the others' weights of 2e-9 to 4e-8 leave: all of them count. As many units as CTAs, so that none is cut.
+    # Beyond the bound of ordinary rows: binary16 holds a weight times 2^7 at least, and a number below its smallest
+    # normal one is off by 2^-25 at most, so each of N positions adds 2^-32 of its |v| to the error, and the result
+    # is such a number too.
+    kv, n_kv = 2000, 148
+    B = Batch([(n, kv)], n_kv, 64, 64, typ, 300)
+    g = torch.Generator().manual_seed(301)
+    k, v = torch.rand(kv, generator=g) * 0.375 - 0.25, 1 + torch.rand(kv, generator=g)
+    k[0], v[0] = 2.25, 0.0  # a score of 18 beside scores of -2 to 1
+    place(B, 0, 0, kv, k=k, v=v)
+    q = queries(B, 2 * n_kv)
+    out = torch.zeros_like(q)
+    want, mag, big = B.attention(q, 2 * n_kv, 0.125, out)
+    call(gb, kernels, B, q, 2 * n_kv, 0.125, out)
+    torch.cuda.synchronize()
+    tol = bound(typ, 64, kv, want, mag, big) + (kv * 2.0 ** -32 * 2 + 2.0 ** -25 if typ == "f16" else 0)
+    assert (tol < 0.2 * want).all()  # the bound tells a result from none
+    assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() / want).max())

@@ -289,7 +289,12 @@ GB_DEV long long pool_row(const ChunkArgs &a, const Seq &s, int b, int h, int p,
 // within (which = 0) and the one it begins and does not end (which = 1). Each
 // place holds kMaxHD floats of RU rows, four
 // dimensions of all rows after another (a warp's rows store 512 bytes at a
-// time), then the rows' maxima (of the scores in powers of two) and sums.
+// time), then what the rows' powers of two are taken from (their maxima, or
+// near them) and their sums, kUnseen where a row sees no position of the
+// piece: what lies there of its output is nothing of the row's, and is left
+// out. A piece is not left out for a weight of zero, which does not stop a NaN
+// in V that the row sees, wherever the line is cut.
+constexpr float kUnseen = -1.f;
 constexpr int kMaxHD = 128, kPlaces = 2;
 template <int RU>
 GB_DEV float *part_slot(const ChunkArgs &a, int cta, int which) {
@@ -435,12 +440,14 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = 0; i0 < n; i0 += 32) {
-      float mi = -INFINITY, l_i = 0.f;
+      float mi = -INFINITY, l_i = kUnseen;
       const int i = i0 + lane;
       if (i < n) {
         const float *p = part + ((uint32_t)i * kStep + (i ? 0 : kPlace) + RU * kMaxHD + r);
         mi = __ldcg(p), l_i = __ldcg(p + RU);
       }
+      const unsigned seen = __ballot_sync(0xffffffffu, l_i != kUnseen);
+      if (l_i == kUnseen) l_i = 0.f;
       const float mn = fmaxf(m, gb_warp_max(mi)), ms = mn == -INFINITY ? 0.f : mn, g = ex2(m - ms), e = ex2(mi - ms);
       l = l * g + gb_warp_sum(e * l_i);
       o.x *= g, o.y *= g, o.z *= g, o.w *= g;
@@ -451,8 +458,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
       for (int j = 0; j < many; j++) {
         const float4 v = __ldcg(p + (j * kStep + (i0 + j ? 0 : kPlace)) / 4);
         const float ej = __shfl_sync(0xffffffffu, e, j);
-        // a weight of zero: nothing seen there, and what lies there may not have been written
-        if (ej != 0.f) o.x = fmaf(ej, v.x, o.x), o.y = fmaf(ej, v.y, o.y), o.z = fmaf(ej, v.z, o.z), o.w = fmaf(ej, v.w, o.w);
+        if (seen >> j & 1) o.x = fmaf(ej, v.x, o.x), o.y = fmaf(ej, v.y, o.y), o.z = fmaf(ej, v.z, o.z), o.w = fmaf(ej, v.w, o.w);
       }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -480,8 +486,8 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
         for (int i = li; i < n; i += lanes) {
           const float *p = part + ((uint32_t)i * kStep + (i ? 0 : kPlace) + RU * kMaxHD + r_lo + r);
           const float mi = __ldcg(p), l_i = __ldcg(p + RU), mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
-          f[i * nr + r] = mi;
-          l = l * ex2(m - ms) + l_i * ex2(mi - ms);
+          f[i * nr + r] = l_i == kUnseen ? NAN : mi;  // mi is none
+          l = l * ex2(m - ms) + (l_i == kUnseen ? 0.f : l_i) * ex2(mi - ms);
           m = mn;
         }
       for (int o = 1; o < lanes; o <<= 1) {
@@ -493,7 +499,10 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
       if (m == -INFINITY) m = 0.f;
       const float inv = l != 0.f ? 1.f / l : 0.f;
       if (r < nr)
-        for (int i = li; i < n; i += lanes) f[i * nr + r] = ex2(f[i * nr + r] - m) * inv;
+        for (int i = li; i < n; i += lanes) {
+          const float mi = f[i * nr + r];
+          f[i * nr + r] = isnan(mi) ? kUnseen : ex2(mi - m) * inv;
+        }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
     const int table = (n * nr * 4 + 15) & ~15, pairs = (room - table) / (32 * NT);  // 32-byte pieces a thread holds
@@ -533,8 +542,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
           for (int i = 0; i < many; i++, g += nr, v += 2 * NT) {
             const float4 x = v[0], y = v[NT];
             const float gi = *g;
-            // a weight of zero: nothing seen there, and what lies there may not have been written
-            if (gi != 0.f) {
+            if (gi != kUnseen) {
               o[0] = fmaf(gi, x.x, o[0]), o[1] = fmaf(gi, x.y, o[1]), o[2] = fmaf(gi, x.z, o[2]), o[3] = fmaf(gi, x.w, o[3]);
               o[4] = fmaf(gi, y.x, o[4]), o[5] = fmaf(gi, y.y, o[5]), o[6] = fmaf(gi, y.z, o[6]), o[7] = fmaf(gi, y.w, o[7]);
             }
@@ -730,7 +738,7 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
               make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
         if (tx == 0) {
           dst[ROWS * kMaxHD + r] = m[i];
-          dst[ROWS * (kMaxHD + 1) + r] = l[i];
+          dst[ROWS * (kMaxHD + 1) + r] = visible(w.s, a.G, pr) > w.t0 * TILE ? l[i] : kUnseen;
         }
       }
     }
@@ -1453,7 +1461,7 @@ __global__ void __launch_bounds__(kTN, 1)
         }
         if (!whole && mine && !half && (both || !g)) {
           dst[kTR * kMaxHD + ur] = m;
-          dst[kTR * (kMaxHD + 1) + ur] = l;
+          dst[kTR * (kMaxHD + 1) + ur] = lim > w.t0 * kTT ? l : kUnseen;
         }
         if (odd) *(volatile int *)&sh->odd = 1;
       }

@@ -1,6 +1,8 @@
 """Attention of new rows over the pages where its numbers are at their limits:
 weights far below a row's largest, NaN and infinities that the rows see, units
 of one kind and the other, calls of fewer rows than their sequences bring."""
+import math
+
 import pytest
 import torch
 
@@ -47,3 +49,20 @@ def test_many_small_weights_beside_a_large_one(gb, kernels, cuda, typ, n):
     tol = bound(typ, 64, kv, want, mag, big) + (kv * 2.0 ** -32 * 2 + 2.0 ** -25 if typ == "f16" else 0)
     assert (tol < 0.2 * want).all()  # the bound tells a result from none
     assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() / want).max())
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n", [1, 5, 100])  # joined by a warp a row, and in slices
+@pytest.mark.parametrize("kv", [200, 9000])  # one CTA's piece, and pieces of many
+def test_a_nan_shows_however_small_its_weight(gb, kernels, cuda, typ, n, kv):
+    # position 10 holds NaN in V and weighs 2^-180 of the largest: 0 in float32, and 0 NaN is NaN
+    B = Batch([(n, kv), (1, 300)], 1, 64, 16, typ, 310)
+    low = 64 if kv < 1000 else kv // 2
+    place(B, 0, 0, low, k=-16.0)
+    place(B, 0, low, kv, k=0.0)
+    place(B, 0, 10, 11, v=math.nan)
+    q = queries(B, 4)
+    out = torch.zeros_like(q)
+    call(gb, kernels, B, q, 4, 0.125, out)
+    torch.cuda.synchronize()
+    assert out[:n].isnan().all() and out[n:].isfinite().all()

@@ -369,7 +369,8 @@ GB_DEV void ld4(const void *base, long long i, float *o) {
 // bits (lane = position still, where that is one). Taken for what came out as an
 // infinity or NaN: a tile holds positions that some of its rows do not see, and
 // their weight of zero does not stop a NaN or an infinity in V. Here the row
-// meets nothing but its own positions, so what it shows is its own.
+// meets nothing but its own positions, so what it shows is its own: the NaN of
+// 0 / 0 too, where every score it sees is -infinity.
 template <int T>
 __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, int head, int pr, unsigned mask) {
   const int lane = threadIdx.x & 31, hd = a.c.head_dim, lim = visible(s, a.G, pr);
@@ -437,6 +438,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
   if (hi - lo <= NT / 32) {  // few rows, often of many pieces: a warp to a row, a lane to four dimensions
     const int r = lo + (tid >> 5), lane = tid & 31, pr = w.r0 + r;
     if (r >= hi) return;
+    bool any = false;  // the row sees a piece
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = 0; i0 < n; i0 += 32) {
@@ -447,6 +449,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
         mi = __ldcg(p), l_i = __ldcg(p + RU);
       }
       const unsigned seen = __ballot_sync(0xffffffffu, l_i != kUnseen);
+      any = any || seen;
       if (l_i == kUnseen) l_i = 0.f;
       const float mn = fmaxf(m, gb_warp_max(mi)), ms = mn == -INFINITY ? 0.f : mn, g = ex2(m - ms), e = ex2(mi - ms);
       l = l * g + gb_warp_sum(e * l_i);
@@ -461,7 +464,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
         if (seen >> j & 1) o.x = fmaf(ej, v.x, o.x), o.y = fmaf(ej, v.y, o.y), o.z = fmaf(ej, v.z, o.z), o.w = fmaf(ej, v.w, o.w);
       }
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const float inv = any ? 1.f / l : 0.f;
     o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
     const bool fine = isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w);
     if (4 * lane < hd)
@@ -497,7 +500,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
         m = mn;
       }
       if (m == -INFINITY) m = 0.f;
-      const float inv = l != 0.f ? 1.f / l : 0.f;
+      const float inv = 1.f / l;  // of a row that sees none, not used
       if (r < nr)
         for (int i = li; i < n; i += lanes) {
           const float mi = f[i * nr + r];
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
       const int r = ty + 16 * i, pr = w.r0 + r;
       const bool on = r < w.nr;
       if (whole) {
-        const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
+        const float inv = visible(w.s, a.G, pr) > 0 ? 1.f / l[i] : 0.f;
         const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
         bool odd = false;
 #pragma unroll
@@ -1430,7 +1433,7 @@ __global__ void __launch_bounds__(kTN, 1)
       }
       if (warp_on) {
         const bool two = !both && w.t1 - w.t0 > 1;  // group 1 has had a tile
-        const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
+        const float inv = !whole ? 1.f : lim > 0 ? 1.f / l : 0.f;
         f0 *= inv, f1 *= inv;
         bool odd = false;
         const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;

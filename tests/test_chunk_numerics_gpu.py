@@ -66,3 +66,34 @@ def test_a_nan_shows_however_small_its_weight(gb, kernels, cuda, typ, n, kv):
     call(gb, kernels, B, q, 4, 0.125, out)
     torch.cuda.synchronize()
     assert out[:n].isnan().all() and out[n:].isfinite().all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n,kv", [(1, 1), (1, 700), (1, 9000), (90, 90), (200, 9000)])
+def test_rows_of_scores_minus_infinity(gb, kernels, cuda, typ, n, kv):
+    # every score a row sees is -infinity: its softmax is 0 / 0. A row that sees nothing is zeros all the same.
+    B = Batch([(n, kv), (3, 2), (1, 300)], 2, 64, 16, typ, 320)
+    place(B, 0, 0, kv, k=-math.inf)
+    q = queries(B, 8)
+    out = torch.full_like(q, 7)
+    call(gb, kernels, B, q, 8, 0.125, out)
+    torch.cuda.synchronize()
+    assert out[:n].isnan().all() and (out[n] == 0).all() and out[n + 1:].isfinite().all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_scores_of_minus_infinity_beside_others(gb, kernels, cuda, typ):
+    # the first positions' scores are -infinity: the rows that see no others are NaN, later rows leave them out
+    n = 300
+    B = Batch([(n, n)], 2, 64, 16, typ, 330)
+    q = queries(B, 8)
+    place(B, 0, 0, 5, k=-1000.0)
+    out = torch.zeros_like(q)
+    want, mag, _ = B.attention(q, 8, 0.125, out)  # of a score of -8000: a weight of zero
+    place(B, 0, 0, 5, k=-math.inf)
+    call(gb, kernels, B, q, 8, 0.125, out)
+    torch.cuda.synchronize()
+    pages, slot = B.slots(0, 5, n)
+    big = float(B.k[pages, :, slot].double().abs().sum(-1).max()) * 0.125
+    assert out[:5].isnan().all()
+    assert ((out.double() - want).abs() <= bound(typ, 64, n, want, mag, big))[5:].all()

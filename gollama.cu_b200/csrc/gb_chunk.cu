@@ -46,19 +46,21 @@ struct ChunkArgs {
 // ---- the line of work --------------------------------------------------------
 
 // A sequence as the device data describe it, made safe: rows outside the
-// call's, or a table shorter than kv_len, cannot lead outside the buffers.
+// call's, or a table shorter than kv_len, cannot lead outside the buffers. Its
+// rows stand where the append puts them, at kv_len - q_start[b + 1] + row, also
+// where the call's rows end before the sequence's.
 struct Seq {
   int q0, n;      // first row, new rows
-  int len0;       // positions before the new rows (may be negative: rows that see nothing)
+  int len0;       // position of the first row (may be negative: rows that see nothing)
   int cap;        // positions the sequence holds, at most what its table can name
 };
 GB_DEV Seq seq_of(const ChunkArgs &a, int b) {
   Seq s;
-  const int lo = max(0, a.c.q_start[b]), hi = min(a.c.rows, max(lo, a.c.q_start[b + 1]));
+  const int lo = max(0, a.c.q_start[b]), end = a.c.q_start[b + 1], hi = min(a.c.rows, max(lo, end));
   const int len = a.c.kv_lens[b];
   s.q0 = lo;
   s.n = max(0, hi - lo);
-  s.len0 = max(len, 0) - s.n;
+  s.len0 = s.n ? (int)max((long long)len - end + lo, -(1LL << 30)) : 0;  // n <= 2^30: none of them sees anything from there
   s.cap = min(max(len, 0), a.c.max_pages * a.c.page_size);
   return s;
 }

@@ -97,3 +97,19 @@ def test_scores_of_minus_infinity_beside_others(gb, kernels, cuda, typ):
     big = float(B.k[pages, :, slot].double().abs().sum(-1).max()) * 0.125
     assert out[:5].isnan().all()
     assert ((out.double() - want).abs() <= bound(typ, 64, n, want, mag, big))[5:].all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("rows", [1, 25, 39])
+def test_a_call_of_the_first_rows(gb, kernels, cuda, typ, rows):
+    # the call's rows end within a sequence's: those it has stand where they stand in the whole, as in the append
+    B = Batch([(3, 70), (37, 400)], 2, 64, 16, typ, 340)
+    q = torch.randn((B.rows, 8 * 64), generator=torch.Generator().manual_seed(9)).to(DT[typ]).cuda()
+    out = torch.full_like(q, 7)
+    want, mag, big = B.attention(q, 8, 0.125, out)
+    c = B.chunk(gb)
+    c.rows = rows
+    kernels.attn_chunk_paged(c, q, q.stride(0), 8, 0.125, out, out.stride(0))
+    torch.cuda.synchronize()
+    assert ((out.double() - want).abs() <= bound(typ, 64, 400, want, mag, big))[:rows].all()
+    assert (out[rows:] == 7).all()

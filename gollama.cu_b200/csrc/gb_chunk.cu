@@ -839,6 +839,7 @@ struct TcShared {
   Plan mine;  // this CTA's, for its end
   uint32_t tmem;
   int dead, odd;
+  uint32_t fetched[2];   // ring places up to which K and V were fetched
   Unit unit[2];          // the pieces left in this CTA's places (nr = 0: none)
   int slice[2], busy[2];  // the first row to join of each; whether to come again
   float top[2][2][128];  // what the two threads of a row tell each other
@@ -1176,10 +1177,13 @@ __global__ void __launch_bounds__(kTN, 1)
         __syncwarp();
       }
     }
-    // whatever was fetched has landed before the CTA ends
-    for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) {
+    // Whatever was fetched has landed before the CTA ends. What lies NS and more places before the last fetch has been
+    // read; of the others a slot's last one is waited for, whichever warp it is (another fetch follows a read).
+    if (lane == 0) sh->fetched[kv] = n;
+    asm volatile("bar.sync 14, 64;" ::: "memory");
+    for (uint32_t i = n > NS ? n - NS - 1 : 0; i < n; i++) {
       const uint32_t slot = i % NS;
-      if ((i & 1) != (uint32_t)kv) continue;
+      if ((i & 1) != (uint32_t)kv || i + NS < sh->fetched[(i + NS) & 1]) continue;
       if (ends >> slot & 1) bar_wait(sh, &sh->landed[slot], (phase >> slot & 1) ^ 1, a.err, true);
       else bar_wait(sh, &sh->full[slot], i / NS & 1, a.err, true);
     }

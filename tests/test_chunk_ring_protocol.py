@@ -15,8 +15,6 @@ import random
 
 import pytest
 
-NS = 5
-
 
 class Undefined(Exception):
     pass
@@ -47,10 +45,13 @@ class Barrier:
 
 
 class Block:
-    def __init__(self, pieces, seed, give_up, stops):
+    def __init__(self, pieces, NS, seed, give_up, stops):
+        self.NS = NS  # slots: 5 at head_dim 128, 10 at 64
         self.r, self.give_up, self.stops, self.dead = random.Random(seed), give_up, stops, False
         self.pieces = pieces  # (tiles, whether the last of them is the sequence's end)
         self.full, self.empty, self.ended = ([Barrier() for _ in range(NS)] for _ in range(3))
+        self.fetched = [None, None]
+        self.haste = self.r.choice([1.0, 0.1, 0.01])  # of the copies
         self.flight, self.queue = [], []  # copies on their way; products' reports
 
     def wait(self, bar, parity):
@@ -70,8 +71,10 @@ class Block:
                 yield end and t + 1 == n
 
     def loader(self, kv):
+        NS = self.NS
         n, last = 0, {}
         phase = [0] * NS
+        self.fetched[kv] = None
         for end in self.tiles():
             slot, lap = (n + kv) % NS, (n + kv) // NS
             got = yield from self.wait(self.empty[slot], lap & 1 ^ 1)
@@ -81,21 +84,27 @@ class Block:
             bar.arrive(expect=1)
             self.flight.append(bar)
             if kv and end:
-                last[slot] = (bar, phase[slot])
+                last[n + 1] = (bar, phase[slot])
                 phase[slot] ^= 1
             else:
-                last[slot] = (bar, lap & 1)
-            if not self.stops:  # the older form asked for the slot's own report alone
-                last[slot] = (self.full[slot], lap & 1)
+                last[n + kv] = (bar, lap & 1)
             n += 2
             yield
-        for bar, parity in last.values():  # the last waits are made all the same
-            for _ in range(400):
-                if bar.done(parity):
-                    break
-                yield
+        self.fetched[kv] = n
+        while self.fetched[kv ^ 1] is None:
+            yield
+        for i in range(max(0, n - NS - 1), n):  # the last waits are made all the same
+            if i & 1 == kv and not i + NS < self.fetched[(i + NS) & 1]:
+                bar, parity = last[i]
+                for k in range(4000):
+                    if bar.done(parity):
+                        break
+                    yield
+                else:
+                    raise Undefined("a last wait for nothing")
 
     def zeros(self):
+        NS = self.NS
         n, phase = 0, [0] * NS
         for end in self.tiles():
             if end:
@@ -109,6 +118,7 @@ class Block:
             yield
 
     def products(self):
+        NS = self.NS
         n = 0
         for _ in self.tiles():
             for i in (n, n + 1):
@@ -131,7 +141,8 @@ class Block:
                 except StopIteration:
                     del actors[pick]
             elif self.flight and pick == len(actors):
-                self.flight.pop(self.r.randrange(len(self.flight))).landed()
+                if self.r.random() < self.haste:
+                    self.flight.pop(self.r.randrange(len(self.flight))).landed()
             elif self.queue:
                 self.queue.pop(0).arrive()  # products end in order
         assert not actors
@@ -143,7 +154,8 @@ class Block:
 def blocks(give_up, stops, count):
     for seed in range(count):
         r = random.Random(seed)
-        yield Block([(r.randint(1, 9), r.random() < 0.5) for _ in range(r.randint(1, 6))], seed, give_up, stops)
+        pieces = [(r.randint(1, 9), r.random() < 0.5) for _ in range(r.randint(1, 6))]
+        yield Block(pieces, r.choice([5, 10]), seed, give_up, stops)
 
 
 def test_no_wait_runs_out():

@@ -41,6 +41,7 @@ struct ChunkArgs {
   float *part;        // partial rows (part_slot)
   unsigned *counter;  // [CTAs][kCounters], zero between launches
   unsigned *err;      // a wait ran out (host memory)
+  unsigned polls;     // of a barrier, before a wait runs out
 };
 
 // ---- the line of work --------------------------------------------------------
@@ -937,19 +938,20 @@ GB_DEV uint32_t idesc_of(int N, bool TB) {
 // `tiles`: how many tiles' work the wait spans, of any length in a long sequence.
 // `dead` is looked at each 64th poll: with each of them one sequence decoding took
 // 28.1 us instead of 26.7, and a long chunk 1,060 instead of 1,030.
-GB_DEV bool bar_wait(TcShared *sh, uint64_t *bar, uint32_t parity, unsigned *err, bool last = false, int tiles = 1) {
+GB_DEV bool bar_wait(TcShared *sh, uint64_t *bar, uint32_t parity, const ChunkArgs &a, bool last = false, int tiles = 1) {
+  const uint32_t polls = last ? GB_WAIT_LIMIT : a.polls;
   for (int t = 0; t < tiles; t++)
-    for (uint32_t i = 0; i < GB_WAIT_LIMIT; i++) {
+    for (uint32_t i = 0; i < polls; i++) {
       if (gb_mbar_try_wait(bar, parity)) return true;
       if (!last && (i & 63) == 63 && *(volatile int *)&sh->dead) return false;
     }
   *(volatile int *)&sh->dead = 1;
-  *(volatile unsigned *)err = GB_DEVERR_TIMEOUT;
+  *(volatile unsigned *)a.err = GB_DEVERR_TIMEOUT;
   return false;
 }
 // The same for a warp that fetches: whether it may go on.
-GB_DEV bool fetch_wait(TcShared *sh, uint64_t *bar, uint32_t parity, unsigned *err, int tiles = 1) {
-  return __all_sync(0xffffffffu, bar_wait(sh, bar, parity, err, false, tiles) && !*(volatile int *)&sh->dead);
+GB_DEV bool fetch_wait(TcShared *sh, uint64_t *bar, uint32_t parity, const ChunkArgs &a, int tiles = 1) {
+  return __all_sync(0xffffffffu, bar_wait(sh, bar, parity, a, false, tiles) && !*(volatile int *)&sh->dead);
 }
 
 GB_DEV void cp_async_arrive(uint64_t *bar) {
@@ -1157,7 +1159,7 @@ __global__ void __launch_bounds__(kTN, 1)
         phys = t + 1 < w.t1 && p < w.s.cap ? table[page] : 0;
         const int held = min(max(w.s.cap - t * kTT, 0), kTT), boxes = (held + br - 1) / br;
         const uint32_t slot = (n + kv) % NS;
-        live = fetch_wait(sh, &sh->empty[slot], ((n + kv) / NS & 1) ^ 1, a.err);
+        live = fetch_wait(sh, &sh->empty[slot], ((n + kv) / NS & 1) ^ 1, a);
         if (!live) break;
         // V at the sequence's end goes through the warp that puts the zeros, which then reports it full
         const bool end = kv && held < kTT;
@@ -1184,8 +1186,8 @@ __global__ void __launch_bounds__(kTN, 1)
     for (uint32_t i = n > NS ? n - NS - 1 : 0; i < n; i++) {
       const uint32_t slot = i % NS;
       if ((i & 1) != (uint32_t)kv || i + NS < sh->fetched[(i + NS) & 1]) continue;
-      if (ends >> slot & 1) bar_wait(sh, &sh->landed[slot], (phase >> slot & 1) ^ 1, a.err, true);
-      else bar_wait(sh, &sh->full[slot], i / NS & 1, a.err, true);
+      if (ends >> slot & 1) bar_wait(sh, &sh->landed[slot], (phase >> slot & 1) ^ 1, a, true);
+      else bar_wait(sh, &sh->full[slot], i / NS & 1, a, true);
     }
   } else if (TMA && warp == kSoftWarps + 2) {
     // ---- queries, and zeros over V behind the sequence's end
@@ -1194,7 +1196,7 @@ __global__ void __launch_bounds__(kTN, 1)
     uint32_t n0 = 0, pieces = 0, phase = 0;  // bit i: parity of the next landing in slot i
     int before = 1;                          // tiles of the piece before
     while (w.next(a)) {
-      if (!fetch_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err, before)) break;
+      if (!fetch_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a, before)) break;
       before = w.t1 - w.t0;
       // Where 128 packed rows are whole tokens' heads they are a box: 256 rows took this warp 4.4 us by
       // copies of its own. The box brings rows past the unit's too, which nobody looks at; few rows are copied.
@@ -1217,7 +1219,7 @@ __global__ void __launch_bounds__(kTN, 1)
       const int last = w.s.cap / kTT;  // the tile that the end lies in
       if (last >= w.t0 && last < w.t1) {
         const uint32_t slot = (n0 + 2 * (last - w.t0) + 1) % NS;
-        if (!fetch_wait(sh, &sh->landed[slot], phase >> slot & 1, a.err, before)) break;
+        if (!fetch_wait(sh, &sh->landed[slot], phase >> slot & 1, a, before)) break;
         phase ^= 1u << slot;
         for (int i = (w.s.cap % kTT) * 8 + lane; i < kTT * 8; i += 32)
           for (int c = 0; c < HD / 64; c++)
@@ -1231,7 +1233,7 @@ __global__ void __launch_bounds__(kTN, 1)
       n0 += 2 * (w.t1 - w.t0);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (pieces) bar_wait(sh, &sh->q_full, (pieces - 1) & 1, a.err, true);
+    if (pieces) bar_wait(sh, &sh->q_full, (pieces - 1) & 1, a, true);
   } else if (!TMA && warp >= kSoftWarps && warp < kMmaWarp) {
     // ---- queries, K and V by asynchronous copies
     // A tile's four blocks of 32 rows go round the three warps, one block on with each tile.
@@ -1244,7 +1246,7 @@ __global__ void __launch_bounds__(kTN, 1)
       return t < w.t1 && j < 4 ? pool_row(a, w.s, w.b, w.head, t * kTT + j * 32 + lane, hd) : -1;
     };
     while (live && w.next(a)) {
-      live = fetch_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a.err);
+      live = fetch_wait(sh, &sh->q_empty, (pieces & 1) ^ 1, a);
       if (!live) break;
       load_q(a, w.s, w.r0, w.nr, w.head, q_at, kTile, lw, kLoadWarps, ppr, lane);
       cp_async_arrive(&sh->q_full);
@@ -1256,7 +1258,7 @@ __global__ void __launch_bounds__(kTN, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; kv++, n++) {
           const uint32_t slot = n % NS;
-          live = live && fetch_wait(sh, &sh->empty[slot], (n / NS & 1) ^ 1, a.err);
+          live = live && fetch_wait(sh, &sh->empty[slot], (n / NS & 1) ^ 1, a);
           if (!live) break;
           const uint16_t *pool = (const uint16_t *)(kv ? a.c.v_pool : a.c.k_pool);
           load_rows(pool, at0, ring + slot * kTile, block(t, 0) * 32, ppr, lane);
@@ -1294,7 +1296,7 @@ __global__ void __launch_bounds__(kTN, 1)
       const uint32_t v_at = ring + n % NS * kTile, parity = (g ? np1++ : np0++) & 1;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        bar_wait(sh, &sh->p_full[g][h], parity, a.err);
+        bar_wait(sh, &sh->p_full[g][h], parity, a);
         tc_fence_after();
         if (leader) {
 #pragma unroll
@@ -1316,14 +1318,14 @@ __global__ void __launch_bounds__(kTN, 1)
       __syncwarp();
     };
     auto loaded = [&](uint32_t n) {
-      bar_wait(sh, &sh->full[n % NS], n / NS & 1, a.err);
+      bar_wait(sh, &sh->full[n % NS], n / NS & 1, a);
       // the asynchronous copies' bytes, seen here, before the tensor cores read them (about 400 cycles)
       if (!TMA) gb_fence_proxy_async();
     };
     while (w.next(a)) {
       const int n = w.t1 - w.t0;
       const bool both = w.nr > 128;  // both groups use each tile
-      bar_wait(sh, &sh->q_full, pieces & 1, a.err);
+      bar_wait(sh, &sh->q_full, pieces & 1, a);
       gb_fence_proxy_async();
       loaded(n0);
       if (both) {
@@ -1336,7 +1338,7 @@ __global__ void __launch_bounds__(kTN, 1)
           qk(1, 0, n0 + 2, true, n == 2);
         }
       }
-      bar_wait(sh, &sh->o_free, (pieces & 1) ^ 1, a.err);  // O of the last unit has been read
+      bar_wait(sh, &sh->o_free, (pieces & 1) ^ 1, a);  // O of the last unit has been read
       for (int t = 0; t < n; t++) {
         const uint32_t v = n0 + 2 * t + 1;
         loaded(v);
@@ -1361,7 +1363,7 @@ __global__ void __launch_bounds__(kTN, 1)
     // nothing is in flight when the tensor memory is given back
     if (leader) tc_commit(&sh->fin);
     __syncwarp();
-    bar_wait(sh, &sh->fin, 0, a.err, true);
+    bar_wait(sh, &sh->fin, 0, a, true);
   } else {
     // ---- softmax: two threads to a row
     const int g = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
@@ -1380,7 +1382,7 @@ __global__ void __launch_bounds__(kTN, 1)
       float m = -INFINITY, l = 0.f;
       int done = 0;
       for (int t = w.t0 + (both ? 0 : g); t < w.t1; t += both ? 1 : 2, ns++, done++) {
-        bar_wait(sh, &sh->s_full[g], ns & 1, a.err);
+        bar_wait(sh, &sh->s_full[g], ns & 1, a);
         tc_fence_after();
         if (warp_on) {
           // the scores are read twice, once for the maximum and once for P: kept in
@@ -1412,7 +1414,7 @@ __global__ void __launch_bounds__(kTN, 1)
             const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
             l *= f;
             if (done) {  // O is there: the last P V must have ended before it is scaled
-              bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
+              bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a);
               tc_fence_after();
               for (int c = half; c < hd / 16; c += 2) {
                 const uint32_t o_at = tmem + 256 + g * 128 + lanes + 16 * c;
@@ -1438,7 +1440,7 @@ __global__ void __launch_bounds__(kTN, 1)
       // keep step: none reports O free twice before another has once.
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       if (done) {
-        bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a.err);
+        bar_wait(sh, &sh->pv_done[g], (ns - 1) & 1, a);
         tc_fence_after();
       }
       float f0 = 1.f, f1 = 0.f;  // weights of this group's result (both), or of the two groups'
@@ -1686,7 +1688,7 @@ int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, i
 }
 
 int gb_attn_chunk_launch(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale, void *out,
-                         long long ldo, float *part, unsigned *counter, unsigned *err, int sms,
+                         long long ldo, float *part, unsigned *counter, unsigned *err, unsigned polls, int sms,
                          cudaStream_t st) {
   const char *what = "gpu: chunk attention";
   ChunkArgs a = {};
@@ -1694,7 +1696,7 @@ int gb_attn_chunk_launch(const gb_paged_chunk *c, const void *q, long long ldq, 
   a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
   a.n_heads = n_heads, a.G = n_heads / c->n_kv;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  a.part = part, a.counter = counter, a.err = err;
+  a.part = part, a.counter = counter, a.err = err, a.polls = polls;
   if (c->kv_typ == GB_F32)
     return c->head_dim <= 64 ? launch_f32<64>(a, 2 * sms, st, what) : launch_f32<128>(a, 2 * sms, st, what);
   if (c->kv_typ == GB_F16) return launch_16<GB_F16>(a, sms, st, what);

@@ -253,7 +253,7 @@ int gb_attn_chunk_counters(int sms);
 int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale,
                         const void *out, long long ldo);
 int gb_attn_chunk_launch(const gb_paged_chunk *c, const void *q, long long ldq, int n_heads, float scale, void *out,
-                         long long ldo, float *part, unsigned *counter, unsigned *err, int sms,
+                         long long ldo, float *part, unsigned *counter, unsigned *err, unsigned polls, int sms,
                          cudaStream_t st);
 
 // gb_sample.cu: one token from logits[n]; parameters by value (p_host) or

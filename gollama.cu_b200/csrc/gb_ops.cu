@@ -499,6 +499,7 @@ struct gb_kernels {
   size_t pws_counters = 0;
   float *cws = nullptr;  // chunk attention: partial rows + counters, one allocation of a fixed size
   unsigned *cerr = nullptr;  // its error word, in page-locked host memory the kernel writes to
+  unsigned cpolls = GB_WAIT_LIMIT;  // polls of its waits
   int sms = 0;
 };
 
@@ -992,6 +993,13 @@ int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *
                                      k != nullptr, (cudaStream_t)stream);
 }
 
+// Whether a wait of the handle's chunk attention has run out since it was last asked.
+static int chunk_status(gb_kernels *k) {
+  if (!k->cerr || !*(volatile unsigned *)k->cerr) return GB_OK;
+  *(volatile unsigned *)k->cerr = 0;
+  return gb_fail(GB_ERR_TIMEOUT, "gpu: chunk attention: a wait in an earlier call ran out; its results are not valid");
+}
+
 int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, const void *q, int64_t ldq,
                             int n_heads, float scale, void *out, int64_t ldo) {
   gb_clear_error();
@@ -1001,10 +1009,8 @@ int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c
   if (!c->rows || !c->batch) return GB_OK;
   const OnDevice on(k);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (k->cerr && *(volatile unsigned *)k->cerr) {
-    *k->cerr = 0;
-    return gb_fail(GB_ERR_TIMEOUT, "gpu: chunk attention: a wait in an earlier call ran out; its results are not valid");
-  }
+  const int before = chunk_status(k);
+  if (before != GB_OK) return before;
   const size_t floats = gb_attn_chunk_part_floats(k->sms);
   if (!k->cws) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -1028,7 +1034,22 @@ int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c
     k->cws = ws;
   }
   return gb_attn_chunk_launch(c, q, ldq, n_heads, scale, out, ldo, k->cws, (unsigned *)(k->cws + floats),
-                              k->cerr, k->sms, st);
+                              k->cerr, k->cpolls, k->sms, st);
+}
+
+int gb_gpu_attn_chunk_status(gb_kernels *k) {
+  gb_clear_error();
+  GB_NEED(k);
+  return chunk_status(k);
+}
+
+int gb_gpu_attn_chunk_wait_limit(gb_kernels *k, int64_t polls) {
+  gb_clear_error();
+  if (polls > (int64_t)GB_WAIT_LIMIT)
+    return gb_fail(GB_ERR_INVALID, "gpu: chunk attention: a limit of %lld polls (%u at most)", (long long)polls, GB_WAIT_LIMIT);
+  GB_NEED(k);
+  k->cpolls = polls < 0 ? GB_WAIT_LIMIT : (unsigned)polls;
+  return GB_OK;
 }
 
 // model.Argmax, model/model.go:376.

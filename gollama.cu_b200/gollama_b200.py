@@ -131,7 +131,8 @@ _SIGS = {
     "gb_gpu_attn_decode_paged": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, F, P]),
     "gb_gpu_qk_norm_rope": (I, [P, P, I, P, I64, I, P, I64, I, I, I, P, P, P, I, P, I64, P, I64]),
     "gb_gpu_rope_append_paged": (I, [P, P, P, I, P, I64, I, P, I64, P, I64, P, P, P, I64]),
-    "gb_gpu_attn_chunk_paged": (I, [P, P, P, P, I64, I, F, P, I64]),
+    "gb_gpu_attn_chunk_paged": (I, [P, P, P, P, I64, I, F, P, I64]), "gb_gpu_attn_chunk_status": (I, [P]),
+    "gb_gpu_attn_chunk_wait_limit": (I, [P, I64]),
     "gb_model_set_sampler": (I, [P, P]), "gb_model_prefill": (I, [P, P, I, I, P]),
     "gb_model_cache_f16_weights": (I, [P, C.POINTER(S)]),
     "gb_linear_matmul_f16": (I, [P, P, P, I, P]), "gb_linear_cache_f16_weights": (I, [P, C.POINTER(S)]),
@@ -323,6 +324,15 @@ class Kernels:
         """gb_gpu_attn_chunk_paged: attention of the new rows over their sequences' pages."""
         _check(lib().gb_gpu_attn_chunk_paged(self.h, _stream(stream), _ref(chunk), _ptr(q), ldq, n_heads, scale,
                                              _ptr(out), ldo))
+
+    def attn_chunk_status(self):
+        """gb_gpu_attn_chunk_status: raises GB_ERR_TIMEOUT once where a wait of attn_chunk_paged, called or replayed,
+        has run out. After a synchronization."""
+        _check(lib().gb_gpu_attn_chunk_status(self.h))
+
+    def attn_chunk_wait_limit(self, polls=-1):
+        """gb_gpu_attn_chunk_wait_limit: polls after which a wait runs out (negative: the default)."""
+        _check(lib().gb_gpu_attn_chunk_wait_limit(self.h, polls))
 
     def sample(self, logits, n, params: SampleParams, recent, n_recent, counter, out, stream=None):
         _check(lib().gb_gpu_sample(self.h, _stream(stream), _ptr(logits), n, C.byref(params),

@@ -242,10 +242,20 @@ int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *
  * allocates it (so not inside a stream capture: GB_ERR_INVALID) and it never
  * moves. Calls on one `k` must not overlap on the GPU; use a handle for each
  * of several streams. The kernel's waits are bounded: should one run out, the
- * call ends with undefined outputs and the handle's next call of this function
- * returns GB_ERR_TIMEOUT. */
+ * call ends with undefined outputs and gb_gpu_attn_chunk_status tells. */
 int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, const void *q, int64_t ldq,
                             int n_heads, float scale, void *out, int64_t ldo);
+/* Whether a wait ran out in any of the handle's gb_gpu_attn_chunk_paged launches,
+ * replays of captured ones included, since this was last told: GB_ERR_TIMEOUT
+ * once, then GB_OK again. It neither launches nor waits: ask after the stream
+ * (or the graph's) has been synchronized. The next call of
+ * gb_gpu_attn_chunk_paged asks too, and where it finds so returns
+ * GB_ERR_TIMEOUT in place of its own launch. */
+int gb_gpu_attn_chunk_status(gb_kernels *k);
+/* The polls after which a wait of the handle's launches from here on runs out
+ * (a captured launch keeps its limit): 2^20 at most, as a negative number
+ * restores; 0 lets every wait run out, to try what a program does then. */
+int gb_gpu_attn_chunk_wait_limit(gb_kernels *k, int64_t polls);
 
 /* ---- sampling (added; the reference's roadmap item, ROADMAP.md:42-45) ----
  * One token from a logits vector on the device:

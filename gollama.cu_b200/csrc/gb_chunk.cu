@@ -1678,6 +1678,7 @@ int gb_attn_chunk_check(const gb_paged_chunk *c, const void *q, long long ldq, i
   if (n_heads > (1 << 16) || (long long)c->rows * (n_heads / c->n_kv) > (1LL << 30))
     return gb_fail(GB_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what, c->rows, n_heads);
   if (!(scale > 0.f) || isinf(scale)) return gb_fail(GB_ERR_INVALID, "%s: scale %g", what, scale);
+  if (!gb_paged_chunk_any(c)) return GB_OK;
   if (!q || !out || (((uintptr_t)q | (uintptr_t)out) & 15))
     return gb_fail(GB_ERR_INVALID, "%s: q or out is null or not on a 16-byte boundary", what);
   const long long wide = (long long)n_heads * hd;

@@ -237,6 +237,9 @@ int gb_argmax_rows_launch(const float *x, int rows, int n, int32_t *out, cudaStr
 // gb_rows.cu: per-head norms, rotation and the append to the pages. Arguments are
 // checked before `loaded` (a handle was given), so refusals need no device.
 int gb_paged_chunk_check(const char *what, const gb_paged_chunk *c);
+// Whether there is anything to do: without rows or sequences no buffer is looked
+// at, and an empty one's address may be null.
+inline bool gb_paged_chunk_any(const gb_paged_chunk *c) { return c->rows && c->batch; }
 int gb_qk_norm_rope_launch(int typ, const void *q, long long ldq, int n_heads, const void *k, long long ldk, int n_kv,
                            int rows, int head_dim, const gb_qk_norm_params *norm, const gb_rope_params *rope,
                            const int32_t *pos, int out_typ, void *q_out, long long ldqo, void *k_out, long long ldko,

@@ -1006,7 +1006,7 @@ int gb_gpu_attn_chunk_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c
   const int rc = gb_attn_chunk_check(c, q, ldq, n_heads, scale, out, ldo);
   if (rc != GB_OK) return rc;
   GB_NEED(k);
-  if (!c->rows || !c->batch) return GB_OK;
+  if (!gb_paged_chunk_any(c)) return GB_OK;
   const OnDevice on(k);
   const cudaStream_t st = (cudaStream_t)stream;
   const int before = chunk_status(k);

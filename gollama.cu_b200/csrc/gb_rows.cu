@@ -385,12 +385,12 @@ int gb_qk_norm_rope_launch(int typ, const void *q, long long ldq, int n_heads, c
   RowArgs a = {};
   GB_TRY(common(what, a, n_heads, n_kv, 0, head_dim, rows, norm, rope));
   if (!known(typ) || !known(out_typ)) return gb_fail(GB_ERR_UNSUPPORTED, "%s: types %d and %d", what, typ, out_typ);
-  if (a.dims && !pos) return gb_fail(GB_ERR_INVALID, "%s: pos is null", what);
-  if (n_heads) {
+  if (rows && a.dims && !pos) return gb_fail(GB_ERR_INVALID, "%s: pos is null", what);
+  if (rows && n_heads) {
     GB_TRY(check_rows(what, "q", q, ldq, n_heads, head_dim, rows));
     GB_TRY(check_rows(what, "q_out", q_out, ldqo, n_heads, head_dim, rows));
   }
-  if (n_kv) {
+  if (rows && n_kv) {
     GB_TRY(check_rows(what, "k", k, ldk, n_kv, head_dim, rows));
     GB_TRY(check_rows(what, "k_out", k_out, ldko, n_kv, head_dim, rows));
   }
@@ -405,12 +405,12 @@ int gb_qk_norm_rope_launch(int typ, const void *q, long long ldq, int n_heads, c
 int gb_paged_chunk_check(const char *what, const gb_paged_chunk *c) {
   if (!c) return gb_fail(GB_ERR_INVALID, "%s: no chunk", what);
   if (c->rows < 0 || c->batch < 0 || c->max_pages <= 0 || c->n_pages <= 0 || c->page_size <= 0 || c->n_kv <= 0 ||
-      c->n_kv > (1 << 16) || !c->q_start || !c->kv_lens || !c->block_table)
+      c->n_kv > (1 << 16) || (gb_paged_chunk_any(c) && (!c->q_start || !c->kv_lens || !c->block_table)))
     return gb_fail(GB_ERR_INVALID, "%s: bad arguments", what);
   if ((long long)c->max_pages * c->page_size > 0x7FFFFF00LL)
     return gb_fail(GB_ERR_INVALID, "%s: %d pages of %d positions for a sequence", what, c->max_pages, c->page_size);
   if (!known(c->kv_typ)) return gb_fail(GB_ERR_UNSUPPORTED, "%s: pool type %d", what, c->kv_typ);
-  if (!c->k_pool || !c->v_pool || (((uintptr_t)c->k_pool | (uintptr_t)c->v_pool) & 15))
+  if ((gb_paged_chunk_any(c) && (!c->k_pool || !c->v_pool)) || (((uintptr_t)c->k_pool | (uintptr_t)c->v_pool) & 15))
     return gb_fail(GB_ERR_INVALID, "%s: pools are null or not on a 16-byte boundary", what);
   return GB_OK;
 }
@@ -424,14 +424,17 @@ int gb_rope_append_paged_launch(const gb_paged_chunk *c, int typ, const void *q,
   RowArgs a = {};
   GB_TRY(common(what, a, n_heads, c->n_kv, c->n_kv, c->head_dim, c->rows, norm, rope));
   if (!known(typ)) return gb_fail(GB_ERR_UNSUPPORTED, "%s: type %d", what, typ);
-  if (n_heads) {
+  const bool any = gb_paged_chunk_any(c);
+  if (any && n_heads) {
     GB_TRY(check_rows(what, "q", q, ldq, n_heads, c->head_dim, c->rows));
     GB_TRY(check_rows(what, "q_out", q_out, ldqo, n_heads, c->head_dim, c->rows));
   }
-  GB_TRY(check_rows(what, "k", k, ldk, c->n_kv, c->head_dim, c->rows));
-  GB_TRY(check_rows(what, "v", v, ldv, c->n_kv, c->head_dim, c->rows));
+  if (any) {
+    GB_TRY(check_rows(what, "k", k, ldk, c->n_kv, c->head_dim, c->rows));
+    GB_TRY(check_rows(what, "v", v, ldv, c->n_kv, c->head_dim, c->rows));
+  }
   if (!loaded) return gb_fail(GB_ERR_INVALID, "gpu: kernels not loaded");
-  if (!c->rows || !c->batch) return GB_OK;
+  if (!any) return GB_OK;
   a.q = q, a.k = k, a.v = v, a.q_out = q_out;
   a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldqo = ldqo;
   a.c = *c;

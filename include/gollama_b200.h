@@ -175,7 +175,8 @@ int gb_gpu_peer_resid_tagged(gb_kernels *k, void *stream, int world, const unsig
  * the new rows. Types are GB_F32, GB_F16 or GB_BF16. Every operand lies on a
  * 16-byte boundary with its rows (tokens) ld* elements apart, a multiple of 8;
  * a row's heads are contiguous. Launches go to `stream` on the device of `k`,
- * whichever device is current. */
+ * whichever device is current. Without rows (or sequences) nothing is done, and
+ * buffers may be null. */
 
 /* The rotation (cpu.RoPE, backend/cpu/cpu.go:118): the first `dims` elements
  * of a head (a multiple of 16; 0: none) in pairs (2j, 2j+1), or (j, j + dims/2)

@@ -140,14 +140,13 @@ GB_DEV void rows_landed(int n) {
 // R rows by a slice of their heads to a CTA, a thread to the same 16 elements of
 // a head in each row: all rows' elements are on their way while the rows'
 // sequences are looked up (by each warp for itself) and their R dims/2 angles
-// formed, once for all heads. R is 1, or 4 for norms of 2^26 elements and more in 16 bits,
-// the elements then on their way to shared memory, where a thread reads what it
-// asked for. 8192 rows of 72 heads of 128 take 59 us so, 5.1 TB/s of what they
-// read and write, and 64 with a CTA to a row; of 40 heads 36 either way; with
-// float32 rows, of which two fit, 60 against 43, and the append of 8192 rows of
-// 48 heads 33.5 against 31. CTAs of up to 192 threads: 320 took 66, 37, 47 and
-// 31, 128 took 64, 40, 46 and 30.5. Few rows are bound by the launch: 2.3 us for
-// one, 3 for 64 with their append (launches of one graph).
+// formed, once for all heads. R is 1, or 4 by the rule of four_rows(), the
+// elements then on their way to shared memory, where a thread reads what it
+// asked for. With float32 rows, of which two fit, 8192 rows of 40 heads took 60
+// us against 43, and the append of 8192 rows of 48 heads 33.5 against 31. CTAs of
+// up to 192 threads: 320 took 66, 37, 47 and 31, 128 took 64, 40, 46 and 30.5.
+// Few rows are bound by the launch: 2.3 us for one, 3 for 64 with their append
+// (launches of one graph).
 template <int TI, int TO, bool APPEND, int R>
 __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 5 : 1) head_rows_kernel(const __grid_constant__ RowArgs a) {
   static_assert(R == 1 || (sizeof(Raw<TI>) == 16 && !APPEND), "rows by way of shared memory");
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 5 : 1) head_rows_kernel(c
     }
     if (!k.on || !(rows_there >> i & 1)) continue;
     if (k.rot) {
-      if (a.halves) {
+      if (R > 1 || a.halves) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const float2 c = cs[i][e * eighth + l8];
@@ -289,14 +288,31 @@ __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 5 : 1) head_rows_kernel(c
   }
 }
 
+// Whether CTAs of four rows are the quicker ones: rows in and out of 16 bits, each
+// head turned as a whole in halves, head_dim up to 128, CTAs of 128 threads and
+// more, and of them six times the 740 that fit the GPU at once. From there on four rows share
+// the angles, which one row's threads wait for. Measured in graphs over 400 MB
+// and more, heads x head_dim: rows, us for one row | four: 72 x 128: 6,000, 47.8 |
+// 45.8; 8,192, 65.3 | 60.6; 32,768, 249 | 220. 72 x 64: 12,000, 48.3 | 44.9. 72 x
+// 96: 8,192, 61.4 | 55.4. 40 x 128: 12,000, 52.0 | 50.5; 32,768, 134 | 125. 32 x
+// 128: 13,000, 44.9 | 44.2. 32 x 64: 32,768, 53.3 | 49.2. 288 x 128: 2,048, 63.5 |
+// 60.2; without norms 72 x 128: 8,192, 55.1 | 48.2. On the other side, 72 x 128
+// but for what is said: 2,048 rows, 18.2 | 19.5; 4,096, 33.1 | 32.8; 40 x 128: 8,192,
+// 35.9 | 36.0; pairs side by side: 8,192, 77.9 | 91.4; norms alone: 67.1 | 88.0;
+// 64 of 128 dims turned: 70.3 | 72.6; to float32: 80.4 | 79.7, 32 heads of 32,768
+// rows 137 | 144; 40 x 256: 16,384, 144 | 146; 4 x 128 (CTAs of 32 threads): 131,072, 77.8 | 82.7.
+bool four_rows(const RowArgs &a, int threads, int slices) {
+  return a.halves && a.dims == a.hd && a.hd <= 128 && threads >= 128 && (long long)(a.rows + 3) / 4 * slices >= 6 * 740;
+}
+
 template <int I, int O, bool APPEND>
 int launch_types(const RowArgs &a, cudaStream_t st, const char *what) {
   // a task to a thread: slices of the heads beside one another
   const int tasks = (a.nq + a.nk + a.nv) << a.lph_log2, slices = (tasks + kMaxThreads - 1) / kMaxThreads;
   const int threads = ((tasks + slices - 1) / slices + 31) / 32 * 32;
-  if constexpr (!APPEND && I != GB_F32) {
+  if constexpr (!APPEND && I != GB_F32 && O != GB_F32) {
     constexpr int R = 4;
-    if ((long long)a.rows * (a.nq + a.nk) * a.hd >= 1 << 26) {
+    if (four_rows(a, threads, slices)) {
       const int smem = R * threads * 2 * (int)sizeof(Raw<I>);
       GB_CUDA(cudaFuncSetAttribute(head_rows_kernel<I, O, APPEND, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
       head_rows_kernel<I, O, APPEND, R>

@@ -182,16 +182,13 @@ __global__ void __launch_bounds__(kMaxThreads, R > 1 ? 5 : 1) head_rows_kernel(c
   const int row = row0 + lane;
   bool there = lane < R && row < a.rows;
   long long p = 0, slot = -1;
-  if constexpr (APPEND) {
+  if constexpr (APPEND) {  // one row: lane 0's
     int b = -1;
     for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
       const bool in = b0 + lane < a.c.batch;
       const int lo = in ? a.c.q_start[b0 + lane] : 0, hi = in ? a.c.q_start[b0 + lane + 1] : 0;
-#pragma unroll
-      for (int i = 0; i < R; i++) {
-        const unsigned hit = __ballot_sync(0xffffffffu, lo <= row0 + i && row0 + i < hi);
-        if (lane == i && b < 0 && hit) b = b0 + __ffs(hit) - 1;
-      }
+      const unsigned hit = __ballot_sync(0xffffffffu, lo <= row0 && row0 < hi);
+      if (lane == 0 && b < 0 && hit) b = b0 + __ffs(hit) - 1;
       if (__all_sync(0xffffffffu, !there || b >= 0)) break;
     }
     there = there && b >= 0;

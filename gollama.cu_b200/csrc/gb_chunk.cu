@@ -473,6 +473,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
     if (4 * lane < hd)
       put4<T>(out, (long long)(w.s.q0 + pr / G) * a.ldo + (long long)(w.head * G + pr % G) * hd + 4 * lane, o.x, o.y, o.z, o.w);
     const unsigned odd = __ballot_sync(0xffffffffu, !fine);
+    __syncwarp();  // the stores above come before those of another lane
     if (odd) redo_row<T>(a, w.s, w.b, w.head, pr, odd);
     return;
   }
@@ -733,6 +734,7 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
             put4<GB_F32>(a.out, at + 64 * j + 4 * tx, v[0], v[1], v[2], v[3]);
           }
         const unsigned any = __ballot_sync(0xffffffffu, odd);
+        __syncwarp();  // the stores above come before those of another lane
 #pragma unroll
         for (int half = 0; half < 2; half++)
           if (any >> (16 * half) & 0xFFFFu)

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import DT, Batch
+from serving_ref import DT, Batch, half_step
 from test_chunk_attention_gpu import bound, call
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +113,28 @@ def test_a_call_of_the_first_rows(gb, kernels, cuda, typ, rows):
     torch.cuda.synchronize()
     assert ((out.double() - want).abs() <= bound(typ, 64, 400, want, mag, big))[:rows].all()
     assert (out[rows:] == 7).all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("heads,n", [(1, 1), (4, 1), (4, 32), (128, 1)])
+def test_few_rows_keep_their_weights(gb, kernels, cuda, typ, heads, n):
+    # Up to 128 packed rows hold a weight in two parts of the type: what is left of it is the square of a half step,
+    # nothing of the half step itself. Weights of 1 and 0.7519, which lies between the numbers of both types, on
+    # values that leave little of their sum: the second rounded once (by 7.5e-5 of it in binary16, 2.5e-3 in
+    # bfloat16) would be off by 2.5 times what is allowed here and more.
+    kv = 128
+    B = Batch([(n, kv)], 1, 64, 16, typ, 350)
+    k = torch.zeros(kv, dtype=torch.float64)
+    k[1::2] = -146 / 4096  # exact scores: 0 and -0.28515625
+    v = torch.ones(kv, dtype=torch.float64)
+    v[1::2] = -1.3330
+    place(B, 0, 0, kv, k=k, v=v)
+    q = queries(B, heads)
+    out = torch.zeros_like(q)
+    want, mag, big = B.attention(q, heads, 0.125, out)
+    call(gb, kernels, B, q, heads, 0.125, out)
+    torch.cuda.synchronize()
+    u = half_step(typ)
+    # no error of a score; of a weight the remainder's own half step
+    tol = u * want.abs() + (u * u + 2.0 ** -20 + kv * 2.0 ** -23) * mag
+    assert ((out.double() - want).abs() <= tol).all(), float((out.double() - want).abs().max())

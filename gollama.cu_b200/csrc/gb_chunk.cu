@@ -367,24 +367,90 @@ GB_DEV void ld4(const void *base, long long i, float *o) {
   }
 }
 
-// One row by itself, by one warp: lane = position for the scores, then lane =
-// four dimensions for the sum over V, of which it writes those of the mask's
-// bits (lane = position still, where that is one). Taken for what came out as an
-// infinity or NaN: a tile holds positions that some of its rows do not see, and
-// their weight of zero does not stop a NaN or an infinity in V. Here the row
-// meets nothing but its own positions, so what it shows is its own: the NaN of
-// 0 / 0 too, where every score it sees is -infinity.
+// ---- rows done again -----------------------------------------------------------
+// A tile holds positions that some of its rows do not see, and their weight of
+// zero does not stop a NaN or an infinity in V. So a row that came out with an
+// infinity or NaN is looked at again, by one warp, and where they may be those of
+// others done again by itself.
+struct Unit {
+  Seq s;
+  int b, head, r0, nr, c_first, c_last;
+};
+
+// A lane's four elements (zeros past head_dim) of the pool row at `at`, -1: zeros.
 template <int T>
-__device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, int head, int pr, unsigned mask) {
-  const int lane = threadIdx.x & 31, hd = a.c.head_dim, lim = visible(s, a.G, pr);
-  const long long row = s.q0 + pr / a.G, hq = (long long)(head * a.G + pr % a.G) * hd;
+GB_DEV void lane4(const void *pool, long long at, int hd, float *v) {
+  const int lane = threadIdx.x & 31;
+  const bool there = at >= 0 && 4 * lane < hd;
+  ld4<T>(pool, there ? at + 4 * lane : 0, v);
+  for (int e = 0; e < 4; e++) v[e] = there ? v[e] : 0.f;
+}
+
+// The last position with an infinity or NaN in V among those that the unit's
+// tiles of KT hold and its first row does not see, -1: none.
+template <int T, int KT>
+GB_DEV int last_odd(const ChunkArgs &a, const Unit &w) {
+  const int lane = threadIdx.x & 31, hd = a.c.head_dim, first = visible(w.s, a.G, w.r0);
+  const int end = min(w.s.cap, max(1, (visible(w.s, a.G, w.r0 + w.nr - 1) + KT - 1) / KT) * KT);
+  for (int p0 = end; p0 > first; p0 -= 32) {  // p0 - 1 and down
+    const long long at = p0 - 1 - lane >= first ? pool_row(a, w.s, w.b, w.head, p0 - 1 - lane, hd) : -1;
+    unsigned odd = 0;
+#pragma unroll 8
+    for (int j = 0; j < 32; j++) {
+      float v[4];
+      lane4<T>(a.c.v_pool, __shfl_sync(0xffffffffu, at, j), hd, v);
+      if (!isfinite(v[0]) || !isfinite(v[1]) || !isfinite(v[2]) || !isfinite(v[3])) odd |= 1u << j;
+    }
+    odd = __reduce_or_sync(0xffffffffu, odd);
+    if (odd) return p0 - __ffs(odd);
+  }
+  return -1;
+}
+
+// Whether each NaN of a row's results (this lane's four: r) has to be one: the row
+// sees a NaN in K, or in V at that dimension.
+template <int T>
+GB_DEV bool sees_nan(const ChunkArgs &a, const Unit &w, int lim, float *r) {
+  const int lane = threadIdx.x & 31, hd = a.c.head_dim;
+  if (__any_sync(0xffffffffu, isinf(r[0]) || isinf(r[1]) || isinf(r[2]) || isinf(r[3]))) return false;
+  for (int p0 = 0; p0 < lim; p0 += 32) {
+    const long long at = p0 + lane < lim ? pool_row(a, w.s, w.b, w.head, p0 + lane, hd) : -1;
+    bool nan = false;
+#pragma unroll 4
+    for (int j = 0; j < 32; j++) {
+      const long long pj = __shfl_sync(0xffffffffu, at, j);
+      float v[4], k[4];
+      lane4<T>(a.c.v_pool, pj, hd, v);
+      lane4<T>(a.c.k_pool, pj, hd, k);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (isnan(v[e])) r[e] = 0.f;
+        nan = nan || isnan(k[e]);
+      }
+    }
+    if (__any_sync(0xffffffffu, nan)) return true;
+    if (!__any_sync(0xffffffffu, isnan(r[0]) || isnan(r[1]) || isnan(r[2]) || isnan(r[3]))) return true;
+  }
+  return false;
+}
+
+// A row by itself: lane = position for the scores, then lane = four dimensions
+// for the sum over V, of which it writes those of the mask's bits (lane =
+// position still, where that is one). It meets nothing but its own positions, so
+// what it shows is its own: the NaN of 0 / 0 too, where every score it sees is
+// -infinity.
+template <int T>
+GB_DEV void redo_row(const ChunkArgs &a, const Unit &w, int pr, int lim, unsigned mask) {
+  const int lane = threadIdx.x & 31, hd = a.c.head_dim;
+  const long long row = w.s.q0 + pr / a.G, hq = (long long)(w.head * a.G + pr % a.G) * hd;
   const int c4 = __popc(mask) == 1 ? __ffs(mask) - 1 : -1, my4 = c4 < 0 ? lane : c4;
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = 0; p0 < lim; p0 += 32) {
     const int p = p0 + lane;
-    const long long at = p < lim ? pool_row(a, s, b, head, p, hd) : -1;
+    const long long at = p < lim ? pool_row(a, w.s, w.b, w.head, p, hd) : -1;
     float sc = 0.f;
     if (at >= 0)
+#pragma unroll 8
       for (int d = 0; d < hd; d += 4) {
         float x[4], y[4];
         ld4<T>(a.q, row * a.ldq + hq + d, x);
@@ -397,15 +463,15 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
     m = mn;
     for (int k = 0; k < 4; k++) o[k] *= f;
     const int n = c4 < 0 ? min(32, lim - p0) : 1;
+#pragma unroll 8
     for (int j = 0; j < n; j++) {
       const int from = c4 < 0 ? j : lane;
       const float pj = __shfl_sync(0xffffffffu, e, from);
       const long long vj = __shfl_sync(0xffffffffu, at, from);
-      if (4 * my4 < hd && vj >= 0) {
-        float v[4];
-        ld4<T>(a.c.v_pool, vj + 4 * my4, v);
-        for (int k = 0; k < 4; k++) o[k] = fmaf(pj, v[k], o[k]);
-      }
+      const bool there = 4 * my4 < hd && vj >= 0;
+      float v[4];
+      ld4<T>(a.c.v_pool, there ? vj + 4 * my4 : 0, v);
+      for (int k = 0; k < 4; k++) o[k] = there ? fmaf(pj, v[k], o[k]) : o[k];
     }
   }
   if (c4 >= 0)
@@ -415,13 +481,41 @@ __device__ __noinline__ void redo_row(const ChunkArgs &a, const Seq s, int b, in
     put4<T>(a.out, row * a.ldo + hq + 4 * my4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
+// Looks at a unit's rows [lo, hi), `warps` warps in turn. What came out stands
+// where the unit's tiles hold no infinity or NaN in V that the row does not see (a
+// weight of zero was all that could go wrong; scores that it does not see are
+// replaced), unless its weights had two parts, as an infinity times the remainder
+// may be NaN, and where it has to be NaN in any case: all rows of a prompt done
+// again for one NaN early in its V took 1,900 times a call's 95 us, and take 2
+// times so.
+template <int T, int KT>
+__device__ __noinline__ void redo_rows(const ChunkArgs &a, const Unit w, int lo, int hi, int warp, int warps) {
+  const int lane = threadIdx.x & 31, hd = a.c.head_dim;
+  const bool parts = T != GB_F32 && w.nr <= 128;
+  int last = -2;  // not looked for
+  for (int r = lo + warp; r < hi; r += warps) {
+    const int pr = w.r0 + r, lim = visible(w.s, a.G, pr);
+    const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (4 * lane < hd) {
+      if constexpr (T == GB_F32) {
+        four<T>(__ldcg((const uint4 *)((const float *)a.out + at + 4 * lane)), v);
+      } else {
+        const uint2 x = __ldcg((const uint2 *)((const uint16_t *)a.out + at + 4 * lane));
+        four<T>(make_uint4(x.x, x.y, 0, 0), v);
+      }
+    }
+    const unsigned mask =
+        __ballot_sync(0xffffffffu, !isfinite(v[0]) || !isfinite(v[1]) || !isfinite(v[2]) || !isfinite(v[3]));
+    if (!mask) continue;
+    if (last == -2) last = last_odd<T, KT>(a, w);
+    if ((parts || last >= lim) && !sees_nan<T>(a, w, lim, v)) redo_row<T>(a, w, pr, lim, mask);
+  }
+}
+
 GB_DEV void cp_async16(uint32_t dst, const void *src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-struct Unit {
-  Seq s;
-  int b, head, r0, nr, c_first, c_last;
-};
 
 // Joins the pieces of a unit's rows [lo, hi), CTA by CTA, all NT threads of
 // barrier 1 calling, with `room` bytes of shared memory to work in. First each row's weight of
@@ -429,10 +523,11 @@ struct Unit {
 // the rows, a thread to every so many runs of eight dimensions, whose pieces
 // come through shared memory by asynchronous copies, as many of them on their
 // way as fit: a unit of 256 rows brings 128 KB a piece, and with loads into
-// registers each few of them cost a round trip to L2.
+// registers each few of them cost a round trip to L2. `odd` is set where a result
+// is an infinity or NaN: the caller looks at those rows, its own warps in step.
 template <int T, int RU, int NT>
 __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int tid, uint8_t *smem, int room, int lo,
-                                         int hi) {
+                                         int hi, int *odd) {
   constexpr uint32_t kPlace = RU * (kMaxHD + 2), kStep = kPlaces * kPlace;  // floats of a place, of a CTA's places
   // in registers: through the reference each use is a load of some 200 clocks
   const float *const part = a.part + (uint32_t)w.c_first * kStep;  // piece i at i * kStep, the first in its second place
@@ -472,9 +567,7 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
     const bool fine = isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w);
     if (4 * lane < hd)
       put4<T>(out, (long long)(w.s.q0 + pr / G) * a.ldo + (long long)(w.head * G + pr % G) * hd + 4 * lane, o.x, o.y, o.z, o.w);
-    const unsigned odd = __ballot_sync(0xffffffffu, !fine);
-    __syncwarp();  // the stores above come before those of another lane
-    if (odd) redo_row<T>(a, w.s, w.b, w.head, pr, odd);
+    if (!fine) *(volatile int *)odd = 1;
     return;
   }
   float *const f = (float *)smem;  // [piece][row]
@@ -519,7 +612,6 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
     const int per = NT / nr, sub = tid / nr, r = tid - sub * nr, pr = w.r0 + r_lo + r, n8 = sub < per ? hd / 8 : 0;
     const int token = pr / G;
     const long long at = (long long)(w.s.q0 + token) * a.ldo + (long long)(w.head * G + pr - token * G) * hd;
-    unsigned odd = 0;
     for (int q0 = sub; q0 < n8; q0 += each * per) {
       const int runs = min(each, (n8 - q0 + per - 1) / per);
       auto fetch = [&](int c8, int p0, uint32_t to) {  // pieces p0.. of a run
@@ -559,13 +651,8 @@ __device__ __noinline__ void join_pieces(const ChunkArgs &a, const Unit w, int t
         bool fine = true;
 #pragma unroll
         for (int e = 0; e < 8; e++) fine = fine && isfinite(o[e]);
-        if (!fine) odd |= 3u << 2 * c8;
+        if (!fine) *(volatile int *)odd = 1;
       }
-    }
-    __syncwarp();
-    for (unsigned any = __ballot_sync(0xffffffffu, odd != 0); any; any &= any - 1) {
-      const int from = __ffs(any) - 1;
-      redo_row<T>(a, w.s, w.b, w.head, __shfl_sync(0xffffffffu, pr, from), __shfl_sync(0xffffffffu, odd, from));
     }
     asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");  // the room is used up
   }
@@ -600,12 +687,13 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
   __shared__ Plan plan;
   __shared__ long long prow[2][TILE];
   __shared__ unsigned arrived;
+  __shared__ int odd[2];  // an infinity or NaN in a row of a whole unit, of a joined one
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, hd = a.c.head_dim;
   Walk<ROWS, TILE, 1, 1, 0> w;
   {
     const Plan p = make_plan<ROWS, TILE, 1, 1, 0, kFN>(a, &plan_shared);
     w.start(a, p);
-    if (tid == 0) plan = p;
+    if (tid == 0) plan = p, odd[0] = odd[1] = 0;
   }
   // a tile's rows to shared memory, `row` floats apart; zeros where there is none and past head_dim
   auto fetch = [&](const void *pool, int t, float *to, int row) {
@@ -724,21 +812,16 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
       if (whole) {
         const float inv = visible(w.s, a.G, pr) > 0 ? 1.f / l[i] : 0.f;
         const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
-        bool odd = false;
+        bool fine = true;
 #pragma unroll
         for (int j = 0; j < HD / 64; j++)
           if (on && 64 * j + 4 * tx < hd) {
             float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = o[i][4 * j + k] * inv, odd |= !isfinite(v[k]);
+            for (int k = 0; k < 4; k++) v[k] = o[i][4 * j + k] * inv, fine = fine && isfinite(v[k]);
             put4<GB_F32>(a.out, at + 64 * j + 4 * tx, v[0], v[1], v[2], v[3]);
           }
-        const unsigned any = __ballot_sync(0xffffffffu, odd);
-        __syncwarp();  // the stores above come before those of another lane
-#pragma unroll
-        for (int half = 0; half < 2; half++)
-          if (any >> (16 * half) & 0xFFFFu)
-            redo_row<GB_F32>(a, w.s, w.b, w.head, w.r0 + (tid >> 5) * 2 + half + 16 * i, 0xFFFFFFFFu);
+        if (!fine) *(volatile int *)&odd[0] = 1;
       } else if (on) {
 #pragma unroll
         for (int j = 0; j < HD / 64; j++)
@@ -766,11 +849,18 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
     __syncthreads();
     if (arrived != (unsigned)(c_last - c_first)) continue;
     __threadfence();
-    join_pieces<GB_F32, ROWS, kFN>(a, {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last}, tid, (uint8_t *)sm,
-                                   F::kFloats * (int)sizeof(float), 0, w.nr);
+    const Unit u = {w.s, w.b, w.head, w.r0, w.nr, c_first, c_last};
+    join_pieces<GB_F32, ROWS, kFN>(a, u, tid, (uint8_t *)sm, F::kFloats * (int)sizeof(float), 0, w.nr, &odd[1]);
     __syncthreads();
+    if (odd[1]) redo_rows<GB_F32, TILE>(a, u, 0, w.nr, tid >> 5, kFN / 32);
     if (tid == 0) a.counter[kCounters * c_first] = 0u;  // ready for the next launch
   }
+  __syncthreads();
+  if (!odd[0]) return;
+  w.start(a, plan);
+  while (w.next(a))
+    if (w.t0 == 0 && w.t1 == w.nt)
+      redo_rows<GB_F32, TILE>(a, {w.s, w.b, w.head, w.r0, w.nr, 0, 0}, 0, w.nr, tid >> 5, kFN / 32);
 }
 
 // ---- the kernel on tensor cores (16-bit pools) --------------------------------
@@ -841,7 +931,7 @@ struct TcShared {
   PlanShared plan;
   Plan mine;  // this CTA's, for its end
   uint32_t tmem;
-  int dead, odd;
+  int dead, odd[2];      // a wait ran out; an infinity or NaN in a row of a whole unit, of a joined one
   uint32_t fetched[2];   // ring places up to which K and V were fetched
   Unit unit[2];          // the pieces left in this CTA's places (nr = 0: none)
   int slice[2], busy[2];  // the first row to join of each; whether to come again
@@ -1117,7 +1207,7 @@ __global__ void __launch_bounds__(kTN, 1)
       gb_mbar_init(&sh->q_empty, 1);
       gb_mbar_init(&sh->o_free, kSoftWarps);
       gb_mbar_init(&sh->fin, 1);
-      sh->dead = sh->odd = sh->unit[0].nr = sh->unit[1].nr = 0;
+      sh->dead = sh->odd[0] = sh->odd[1] = sh->unit[0].nr = sh->unit[1].nr = 0;
     }
     gb_mbar_fence_init();
   }
@@ -1503,7 +1593,7 @@ __global__ void __launch_bounds__(kTN, 1)
           dst[kTR * kMaxHD + ur] = m;
           dst[kTR * (kMaxHD + 1) + ur] = lim > w.t0 * kTT ? l : kUnseen;
         }
-        if (odd) *(volatile int *)&sh->odd = 1;
+        if (odd) *(volatile int *)&sh->odd[0] = 1;
       }
       tc_fence_before();
       __syncwarp();
@@ -1542,34 +1632,26 @@ __global__ void __launch_bounds__(kTN, 1)
       }
       __threadfence();
       all();
+      const int lo[2] = {sh->slice[0], sh->slice[1]};
       for (int i = 0; i < 2; i++) {
-        const Unit u = sh->unit[i];
-        const int lo = sh->slice[i];
+        const Unit &u = sh->unit[i];
         // in the tiles' room: all of them are used up
-        if (lo < u.nr)
-          join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid, tc_raw + kHeader, tc_smem<HD>() - kHeader, lo, min(lo + kSlice, u.nr));
+        if (lo[i] < u.nr)
+          join_pieces<T, kTR, kSoftWarps * 32>(a, u, tid, tc_raw + kHeader, tc_smem<HD>() - kHeader, lo[i],
+                                               min(lo[i] + kSlice, u.nr), &sh->odd[1]);
       }
       const bool more = sh->busy[0] || sh->busy[1];
       all();
+      if (sh->odd[1])
+        for (int i = 0; i < 2; i++) redo_rows<T, kTT>(a, sh->unit[i], lo[i], min(lo[i] + kSlice, sh->unit[i].nr), warp, kSoftWarps);
       if (!more) break;
     }
     if (tid < 2 && my_unit->nr && atomicAdd(counter + 2, 1u) == holders - 1) counter[0] = counter[1] = counter[2] = 0u;
-    if (sh->odd) {
+    if (sh->odd[0]) {
       w.start(a, sh->mine);
-      while (w.next(a)) {
-        if (w.t0 != 0 || w.t1 != w.nt) continue;
-        for (int r = warp; r < w.nr; r += kSoftWarps) {
-          const int pr = w.r0 + r;
-          const long long at = (long long)(w.s.q0 + pr / a.G) * a.ldo + (long long)(w.head * a.G + pr % a.G) * hd;
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-          if (4 * lane < hd) {
-            const uint2 x = __ldcg((const uint2 *)((const uint16_t *)a.out + at + 4 * lane));
-            four<T>(make_uint4(x.x, x.y, 0, 0), v);
-          }
-          if (__any_sync(0xffffffffu, !isfinite(v[0]) || !isfinite(v[1]) || !isfinite(v[2]) || !isfinite(v[3])))
-            redo_row<T>(a, w.s, w.b, w.head, pr, 0xFFFFFFFFu);
-        }
-      }
+      while (w.next(a))
+        if (w.t0 == 0 && w.t1 == w.nt)
+          redo_rows<T, kTT>(a, {w.s, w.b, w.head, w.r0, w.nr, 0, 0}, 0, w.nr, warp, kSoftWarps);
     }
   }
   tc_fence_before();

@@ -138,3 +138,58 @@ def test_few_rows_keep_their_weights(gb, kernels, cuda, typ, heads, n):
     # no error of a score; of a weight the remainder's own half step
     tol = u * want.abs() + (u * u + 2.0 ** -20 + kv * 2.0 ** -23) * mag
     assert ((out.double() - want).abs() <= tol).all(), float((out.double() - want).abs().max())
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n,kv", [(256, 4096), (1, 4096)])
+@pytest.mark.parametrize("where", ["one value", "all values", "one key"])
+def test_a_nan_that_all_rows_see_costs_little(gb, kernels, cuda, typ, n, kv, where):
+    # Rows are done again, each by itself, for what a row they share a tile with sees and they do not. A NaN that a
+    # row sees is no reason: all of a prompt's rows done again took 1,900 times a call's time.
+    B = Batch([(n, kv)] * (1 if n > 1 else 16), 8, 128, 16, typ, 360)
+    q = torch.randn((B.rows, 32 * 128), generator=torch.Generator().manual_seed(10)).to(DT[typ]).cuda()
+    out = torch.zeros_like(q)
+
+    def took():
+        best = 1e9
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            call(gb, kernels, B, q, 32, 0.1, out)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    clean = took()
+    assert out.isfinite().all()
+    for b in range(B.batch):
+        if where == "one value":
+            place(B, b, 10, 11, v=math.nan)
+        elif where == "all values":
+            place(B, b, 0, kv, v=math.nan)
+        else:
+            place(B, b, 10, 11, k=math.nan)
+    spoilt = took()
+    assert out.isnan().all()
+    assert spoilt < 20 * clean, (spoilt, clean)
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n,kv", [(1, 300), (100, 300), (100, 3000)])
+def test_an_infinite_value_shows_as_one(gb, kernels, cuda, typ, n, kv):
+    # at one position and in one dimension, with a weight like the others': the rows that see it have it there, and
+    # nothing else changes
+    B = Batch([(n, kv), (2, 50)], 2, 64, 16, typ, 370)
+    q = 0.1 * torch.randn((B.rows, 8 * 64), generator=torch.Generator().manual_seed(11))
+    q, out = q.to(DT[typ]).cuda(), torch.zeros((B.rows, 8 * 64), dtype=DT[typ], device="cuda")
+    want, mag, big = B.attention(q, 8, 0.125, out)
+    at = kv - 1 - n // 2
+    pages, slot = B.slots(0, at, at + 1)
+    B.v[pages, :, slot, 5] = -math.inf
+    call(gb, kernels, B, q, 8, 0.125, out)
+    torch.cuda.synchronize()
+    first = at - (kv - n)
+    shows = out[first:n].reshape(n - first, 8, 64)[..., 5]
+    assert (shows == -math.inf).all()
+    out[first:n].reshape(n - first, 8, 64)[..., 5] = want[first:n].reshape(n - first, 8, 64)[..., 5].to(out.dtype)
+    assert ((out.double() - want).abs() <= bound(typ, 64, kv, want, mag, big)).all()

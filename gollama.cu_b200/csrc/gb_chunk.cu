@@ -486,8 +486,8 @@ GB_DEV void redo_row(const ChunkArgs &a, const Unit &w, int pr, int lim, unsigne
 // weight of zero was all that could go wrong; scores that it does not see are
 // replaced), unless its weights had two parts, as an infinity times the remainder
 // may be NaN, and where it has to be NaN in any case: all rows of a prompt done
-// again for one NaN early in its V took 1,900 times a call's 95 us, and take 2
-// times so.
+// again for one NaN early in its V took 1,900 times a call's 95 us, and looked
+// at like this take 1.7 times.
 template <int T, int KT>
 __device__ __noinline__ void redo_rows(const ChunkArgs &a, const Unit w, int lo, int hi, int warp, int warps) {
   const int lane = threadIdx.x & 31, hd = a.c.head_dim;
@@ -905,10 +905,10 @@ __global__ void __launch_bounds__(kFN, 2) attn_chunk_f32_kernel(const __grid_con
 // that error but the numbers' end: few rows over few outstanding positions do
 // not average it out.
 //
-// Measured in one graph: 64 sequences decoding at 1,200 to 8,000 positions (32
-// heads over 8, head_dim 128) 208 us, 5.8 TB/s of the cache's bytes; 2048 rows of
-// 64 heads behind 14,336 positions 0.89 to 0.93 ms, 1.1 PFLOP/s, the clock held at
-// 1.6 GHz by the power limit. What bounds long chunks is the exchange between a
+// Measured in graphs: 64 sequences decoding at 1,200 to 8,000 positions (32
+// heads over 8, head_dim 128) 214 us, 5.6 TB/s of the cache's bytes, in bursts of
+// 13 ms at 1.97 GHz, and 237 to 247 where the power limit holds the clock at 1.5;
+// 2048 rows of 64 heads behind 14,336 positions 1.01 ms, 1.02 PFLOP/s, under that limit. What bounds long chunks is the exchange between a
 // group's softmax and the products: of a tile's 4,000 clocks the tensor cores
 // work 2,000, and with neither exponentials nor products 2,900 remain.
 constexpr int kTR = 256, kTT = 128;       // rows of a unit, positions of a tile
@@ -1218,7 +1218,8 @@ __global__ void __launch_bounds__(kTN, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // A wide tile takes 4,000 clocks, a narrow one 2,200, and what a piece has before and behind its tiles some 6,000
-  // (counted as 4,000, 12 ragged sequences took 111 us instead of 105; as twice a tile of the unit's kind, 112)
+  // (counted as 4,000, 12 ragged sequences took 111 us instead of 105; as twice a tile of the unit's kind, 112). The
+  // tiles were traced at head_dim 128 with TMA; the other forms are cut by the same costs.
   const Plan plan = make_plan<kTR, kTT, 4, 2, 6, kTN>(a, &sh->plan);
   Walk<kTR, kTT, 4, 2, 6> w;
   w.start(a, plan);
@@ -1469,7 +1470,7 @@ __global__ void __launch_bounds__(kTN, 1)
       const int ur = (both ? g * 128 : 0) + row, pr = w.r0 + ur;
       const bool mine = ur < w.nr;
       const bool warp_on = ur - lane < w.nr;
-      // rows past the unit's in a warp of its rows have zero queries and are not looked at
+      // rows past the unit's in a warp of its rows have zeros for queries, or by TMA other tokens', and are not looked at
       const int lim = mine ? visible(w.s, a.G, pr) : 0x7FFFFFFF;
       float m = -INFINITY, l = 0.f;
       int done = 0;

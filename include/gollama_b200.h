@@ -202,7 +202,8 @@ typedef struct {
  * the device, not decreasing; rows outside [q_start[0], q_start[batch]) belong
  * to no sequence and their outputs are left as they were). kv_lens[b] counts
  * its positions WITH the new rows: the i-th of n rows stands at position
- * kv_lens[b] - n + i. Pools and table are those of gb_gpu_attn_decode_paged:
+ * kv_lens[b] - n + i, n = q_start[b+1] - q_start[b], also where the call's rows
+ * end before the sequence's. Pools and table are those of gb_gpu_attn_decode_paged:
  * k_pool / v_pool = [n_pages][n_kv][page_size][head_dim] of type kv_typ,
  * block_table[batch][max_pages]. */
 typedef struct {
@@ -227,7 +228,8 @@ int gb_gpu_qk_norm_rope(gb_kernels *k, void *stream, int typ, const void *q, int
  * n_heads 0: no queries). A row whose position is negative or past the table,
  * or whose page is outside [0, n_pages), is not appended (its query is still
  * written). Slots no row is appended to keep their contents. Two rows must not
- * share a slot. head_dim is a multiple of 16 up to 256. */
+ * share a slot. head_dim is a multiple of 16 up to 256 (the attention of the
+ * pages, here and in gb_gpu_attn_decode_paged, takes up to 128). */
 int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *c, int typ, const void *q, int64_t ldq,
                              int n_heads, const void *kx, int64_t ldk, const void *v, int64_t ldv,
                              const gb_qk_norm_params *norm, const gb_rope_params *rope, void *q_out, int64_t ldqo);
@@ -235,11 +237,22 @@ int gb_gpu_rope_append_paged(gb_kernels *k, void *stream, const gb_paged_chunk *
  * sequence's positions up to its own, whatever lies in the pages behind
  * kv_lens[b]. q and out [rows][n_heads][head_dim] have the pool's type; a row
  * that sees no position gives zeros. Table entries outside [0, n_pages) read
- * page 0; kv_lens past the table count as the table's length. out overlaps
- * neither q nor the pools. Any number of
+ * page 0; a row that stands past the table's positions sees all of them. out
+ * overlaps neither q nor the pools. Any number of
  * query heads per KV head; head_dim a multiple of 16 up to 128; scale > 0.
  * Float32 statistics and sums; results do not depend on the order in which
- * the GPU runs the parts. Scratch of a fixed size lives in `k`: the first call
+ * the GPU runs the parts. With 16-bit pools the softmax's weights enter the sum
+ * over V rounded to the pool's type, relative to the largest so far, in units
+ * of more than 128 (row, query head of a group) pairs of a sequence: 256 pairs
+ * after another are a unit, so long chunks, but for a last unit of fewer, have
+ * 1.35 times the error that the result's own rounding leaves; units of up to
+ * 128 (decoding) hold them in two parts and have none of it. In binary16 a
+ * weight below 2^-32 of the row's largest is zero.
+ * A NaN or an infinity in the K or V that a row sees shows in it (an infinity
+ * in V as one, or as a NaN where its weight is zero); one that it does not see
+ * does not, but costs: rows that share 128 positions (32 or 64 in float32) or a
+ * unit with it are computed again each by itself, 35 ms for 512 rows at 8,192
+ * positions. Scratch of a fixed size lives in `k`: the first call
  * allocates it (so not inside a stream capture: GB_ERR_INVALID) and it never
  * moves. Calls on one `k` must not overlap on the GPU; use a handle for each
  * of several streams. The kernel's waits are bounded: should one run out, the

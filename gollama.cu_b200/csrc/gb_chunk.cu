@@ -1643,12 +1643,12 @@ __global__ void __launch_bounds__(kTN, 1)
       }
       const bool more = sh->busy[0] || sh->busy[1];
       all();
-      if (sh->odd[1])
+      if (sh->odd[1] && !sh->dead)  // what comes of a wait that ran out is not looked at
         for (int i = 0; i < 2; i++) redo_rows<T, kTT>(a, sh->unit[i], lo[i], min(lo[i] + kSlice, sh->unit[i].nr), warp, kSoftWarps);
       if (!more) break;
     }
     if (tid < 2 && my_unit->nr && atomicAdd(counter + 2, 1u) == holders - 1) counter[0] = counter[1] = counter[2] = 0u;
-    if (sh->odd[0]) {
+    if (sh->odd[0] && !sh->dead) {
       w.start(a, sh->mine);
       while (w.next(a))
         if (w.t0 == 0 && w.t1 == w.nt)
